@@ -150,8 +150,8 @@ BNN_Status BNN_DeviceOpen(uint32_t device_index, BNN_Device* out_device) {
         delete d;
         return BNN_EIO;
     }
-    if (cudaMalloc(&d->d_status, 3 * sizeof(int)) != cudaSuccess ||
-        cudaMemset(d->d_status, 0, 3 * sizeof(int)) != cudaSuccess ||
+    if (cudaMalloc(&d->d_status, bnn::kStatusWords * sizeof(int)) != cudaSuccess ||
+        cudaMemset(d->d_status, 0, bnn::kStatusWords * sizeof(int)) != cudaSuccess ||
         cudaMallocHost(&d->h_status, sizeof(int)) != cudaSuccess) {
         cudaGetLastError();
         if (d->d_status)

@@ -20,7 +20,9 @@ struct bnn_accel_device {
                               // [1], [2] verdicts of single-kernel jobs, used in turn:
                               // each such job clears the other slot for the next one,
                               // so no reset sits between two of them and the next
-                              // job's launch overlaps this one's tail (PDL)
+                              // job's launch overlaps this one's tail (PDL);
+                              // [3] what the paged-cache operators record until
+                              // bnn_b200_paged_sync reads it
     int* h_status;            // pinned host mirror
     int* last_status;         // the verdict word of the last enqueued job
     uint32_t single_jobs;     // single-kernel jobs enqueued (picks the slot)
@@ -58,6 +60,9 @@ extern "C" BNN_Status bnn_b200_matrix_alloc(BNN_Device device, uint32_t in_featu
 void bnn_noalloc_forget(int ordinal);
 
 namespace bnn {
+
+constexpr int kPagedStatusWord = 3;  // index into bnn_accel_device::d_status
+constexpr int kStatusWords = 4;
 
 // Makes `ordinal` current for the lifetime of the guard, restoring the
 // caller's device afterwards.

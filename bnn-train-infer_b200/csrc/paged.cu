@@ -1,0 +1,291 @@
+// paged.cu - host side of the paged-cache operators (include/bnn_b200_paged.h):
+// argument checks, the choice of kernel, launches.
+#include <cmath>
+
+#include "bnn_b200_paged.h"
+#include "bnn_internal.h"
+#include "paged_append.cuh"
+#include "paged_common.cuh"
+
+namespace {
+
+using namespace bnn::paged;
+
+constexpr int64_t kMaxCount = (int64_t)1 << 30;  // tokens, positions, slots
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+BNN_Status check_cache(const BNN_PagedCache& c, Cache* out) {
+    if (c.type != BNN_PAGED_BF16 && c.type != BNN_PAGED_F16)
+        return BNN_EINVAL;
+    if (c.head_dim != 64 && c.head_dim != 128)
+        return BNN_ENOTSUP;
+    uint32_t shift = 0;
+    for (; shift <= 8 && c.page_size != ((int64_t)1 << shift); ++shift) {
+    }
+    if (shift < 4 || shift > 8)
+        return BNN_ENOTSUP;
+    if (c.kv_heads <= 0 || c.kv_heads > 65536 || c.pages <= 0 || c.pages > kMaxCount >> shift)
+        return BNN_EINVAL;
+    if (!c.k || !c.v || !aligned16(c.k) || !aligned16(c.v))
+        return BNN_EINVAL;
+    const int64_t strides[6] = {c.k_page_stride, c.k_head_stride, c.k_row_stride,
+                                c.v_page_stride, c.v_head_stride, c.v_row_stride};
+    for (int64_t s : strides)
+        if (s < c.head_dim || s % 8 != 0 || s >= ((int64_t)1 << 38))
+            return BNN_EINVAL;
+    *out = Cache{static_cast<unsigned char*>(c.k), static_cast<unsigned char*>(c.v), c.k_page_stride, c.k_head_stride,
+                 c.k_row_stride, c.v_page_stride, c.v_head_stride, c.v_row_stride, (uint32_t)c.pages,
+                 (uint32_t)c.kv_heads, shift};
+    return BNN_OK;
+}
+
+// A launch that may start while the stream's previous kernel drains; every
+// kernel here waits for it (griddep_wait) before it reads or writes memory.
+template <typename Args>
+BNN_Status launch(void (*kernel)(Args), dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream, const Args& args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kernel, args) != cudaSuccess) {
+        cudaGetLastError();
+        return BNN_EIO;
+    }
+    return BNN_OK;
+}
+
+// ---- append
+
+template <int D, typename S, typename T, int kHeads>
+BNN_Status launch_append(const AppendArgs& a, bool interleaved, cudaStream_t stream) {
+    constexpr uint32_t heads = kHeads * (128 / D);
+    const uint64_t warps = (uint64_t)a.tokens * ((a.heads + 2 * a.c.kv_heads + heads - 1) / heads);
+    const uint64_t blocks = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    if (blocks > INT32_MAX || warps > UINT32_MAX)
+        return BNN_EINVAL;
+    return launch(interleaved ? append_kernel<D, S, T, true, kHeads> : append_kernel<D, S, T, false, kHeads>,
+                  dim3((uint32_t)blocks), kAppendThreads, 0, stream, a);
+}
+
+template <int D, typename S, typename T>
+BNN_Status append_heads(const AppendArgs& a, bool interleaved, cudaStream_t stream) {
+    return launch_append<D, S, T, 1>(a, interleaved, stream);
+}
+
+template <int D, typename T>
+BNN_Status append_source(const AppendArgs& a, int64_t type, bool interleaved, cudaStream_t stream) {
+    switch (type) {
+    case BNN_PAGED_F32:
+        return append_heads<D, float, T>(a, interleaved, stream);
+    case BNN_PAGED_BF16:
+        return append_heads<D, __nv_bfloat16, T>(a, interleaved, stream);
+    default:
+        return append_heads<D, __half, T>(a, interleaved, stream);
+    }
+}
+
+// ---- attention
+
+// The simple kernel: one warp per (token, query head).
+template <int D, typename T>
+static __global__ void __launch_bounds__(128) attention_rows_kernel(AttnArgs a) {
+    const uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 32;
+    bnn::griddep_launch_dependents();
+    bnn::griddep_wait();
+    const int32_t t = (int32_t)(w / a.heads);
+    if (t >= (int32_t)a.tokens)
+        return;
+    // the last request that starts at or before t
+    uint32_t lo = 0, hi = a.batch;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (a.q_starts[mid] <= t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const Request r = load_request(a, lo);
+    if (t < r.start || t >= r.start + r.n)
+        return;
+    if (r.n > (int32_t)a.max_q) {
+        if ((threadIdx.x & 31) == 0)
+            atomicOr(a.status, kPagedRange);
+        return;
+    }
+    attention_row<D, T>(a, lo, r, t - r.start, (uint32_t)(w % a.heads));
+}
+
+template <int D, typename T>
+BNN_Status attention_typed(const AttnArgs& a, cudaStream_t stream) {
+    const uint64_t blocks = ((uint64_t)a.tokens * a.heads + 3) / 4;
+    if (blocks > INT32_MAX)
+        return BNN_EINVAL;
+    return launch(attention_rows_kernel<D, T>, dim3((uint32_t)blocks), 128, 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc, void* stream) {
+    if (!device || !desc)
+        return BNN_EINVAL;
+    const BNN_PagedAppend& d = *desc;
+    AppendArgs a = {};
+    BNN_Status st = check_cache(d.cache, &a.c);
+    if (st != BNN_OK)
+        return st;
+    if (d.type != BNN_PAGED_F32 && d.type != BNN_PAGED_BF16 && d.type != BNN_PAGED_F16)
+        return BNN_EINVAL;
+    if (d.tokens < 0 || d.tokens > kMaxCount || d.heads <= 0 || d.heads > 65536)
+        return BNN_EINVAL;
+    if (d.rotary_dim < 0 || d.rotary_dim > d.cache.head_dim)
+        return BNN_EINVAL;
+    if (d.rotary_dim % 8 != 0)
+        return BNN_ENOTSUP;
+    if (d.rotary_dim != 0 && (!d.cos || !d.sin || d.table_rows <= 0 || d.table_rows > kMaxCount))
+        return BNN_EINVAL;
+    if (!(d.eps >= 0.0) || !std::isfinite(d.eps) || !aligned16(d.q_norm) || !aligned16(d.k_norm))
+        return BNN_EINVAL;
+    if (d.tokens == 0)
+        return BNN_OK;
+    if (!d.q || !d.k || !d.v || !d.positions || !d.slots || !d.q_out)
+        return BNN_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(d.q_out) & 7u) != 0 || d.out_token_stride % 4 != 0 || d.out_head_stride % 4 != 0)
+        return BNN_EINVAL;
+    a.src[0] = static_cast<const unsigned char*>(d.q);
+    a.src[1] = static_cast<const unsigned char*>(d.k);
+    a.src[2] = static_cast<const unsigned char*>(d.v);
+    a.token[0] = d.q_token_stride;
+    a.token[1] = d.k_token_stride;
+    a.token[2] = d.v_token_stride;
+    a.head[0] = d.q_head_stride;
+    a.head[1] = d.k_head_stride;
+    a.head[2] = d.v_head_stride;
+    a.gain[0] = d.q_norm;
+    a.gain[1] = d.k_norm;
+    a.cos = d.cos;
+    a.sin = d.sin;
+    a.positions = d.positions;
+    a.slots = d.slots;
+    a.q_out = static_cast<unsigned char*>(d.q_out);
+    a.o_token = d.out_token_stride;
+    a.o_head = d.out_head_stride;
+    a.tokens = (uint32_t)d.tokens;
+    a.heads = (uint32_t)d.heads;
+    a.rotary = (uint32_t)d.rotary_dim;
+    a.table_rows = (uint32_t)d.table_rows;
+    a.eps = (float)d.eps;
+    a.status = device->d_status + bnn::kPagedStatusWord;
+    bnn::DeviceGuard guard(device->ordinal);
+    if (!guard.ok())
+        return BNN_EIO;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool wide = d.cache.head_dim == 128, inter = d.interleaved != 0;
+    if (d.cache.type == BNN_PAGED_BF16)
+        return wide ? append_source<128, __nv_bfloat16>(a, d.type, inter, s)
+                    : append_source<64, __nv_bfloat16>(a, d.type, inter, s);
+    return wide ? append_source<128, __half>(a, d.type, inter, s) : append_source<64, __half>(a, d.type, inter, s);
+}
+
+BNN_Status bnn_b200_paged_workspace(BNN_Device device, int64_t batch, int64_t kv_heads, size_t* bytes) {
+    if (!device || !bytes || batch <= 0 || batch > BNN_PAGED_MAX_BATCH || kv_heads <= 0 || kv_heads > 65536)
+        return BNN_EINVAL;
+    *bytes = ((size_t)batch * (size_t)kv_heads * sizeof(int) + 255) & ~(size_t)255;
+    return BNN_OK;
+}
+
+BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention* desc, void* stream) {
+    if (!device || !desc)
+        return BNN_EINVAL;
+    const BNN_PagedAttention& d = *desc;
+    AttnArgs a = {};
+    BNN_Status st = check_cache(d.cache, &a.c);
+    if (st != BNN_OK)
+        return st;
+    if (d.out_type != d.cache.type && d.out_type != BNN_PAGED_F32)
+        return BNN_EINVAL;
+    if (d.batch < 0 || d.tokens < 0 || d.tokens > kMaxCount || d.heads <= 0 || d.max_q < 0 || d.max_q > kMaxCount)
+        return BNN_EINVAL;
+    if (d.batch > BNN_PAGED_MAX_BATCH)
+        return BNN_ENOTSUP;
+    if (d.heads % d.cache.kv_heads != 0)
+        return BNN_EINVAL;
+    if (d.heads / d.cache.kv_heads > BNN_PAGED_MAX_GROUP)
+        return BNN_ENOTSUP;
+    if (d.window < 0 || d.sinks < 0 || !(d.scale > 0.0) || !std::isfinite((float)d.scale) || (float)d.scale == 0.0f)
+        return BNN_EINVAL;
+    if (d.table_width < 0 || d.table_width > kMaxCount || (d.batch > 1 && d.table_stride < d.table_width))
+        return BNN_EINVAL;
+    if (d.batch == 0 || d.tokens == 0 || d.max_q == 0)
+        return BNN_OK;
+    if (!d.q || !d.out || (!d.page_table && d.table_width) || !d.kv_lens || !d.q_starts || !d.workspace)
+        return BNN_EINVAL;
+    size_t need = 0;
+    st = bnn_b200_paged_workspace(device, d.batch, d.cache.kv_heads, &need);
+    if (st != BNN_OK)
+        return st;
+    if (d.workspace_bytes < 0 || (size_t)d.workspace_bytes < need || !aligned16(d.workspace))
+        return BNN_EINVAL;
+    a.q = static_cast<const unsigned char*>(d.q);
+    a.out = static_cast<unsigned char*>(d.out);
+    a.lse = d.lse;
+    a.table = d.page_table;
+    a.kv_lens = d.kv_lens;
+    a.q_starts = d.q_starts;
+    a.q_token = d.q_token_stride;
+    a.q_head = d.q_head_stride;
+    a.o_token = d.out_token_stride;
+    a.o_head = d.out_head_stride;
+    a.lse_token = d.lse_token_stride;
+    a.table_stride = d.table_stride;
+    a.batch = (uint32_t)d.batch;
+    a.tokens = (uint32_t)d.tokens;
+    a.heads = (uint32_t)d.heads;
+    a.group = (uint32_t)(d.heads / d.cache.kv_heads);
+    a.table_width = (uint32_t)d.table_width;
+    a.max_q = (uint32_t)d.max_q;
+    a.window = (uint32_t)(d.window < kMaxCount ? d.window : 0);  // a window past every position is none
+    a.sinks = (uint32_t)(d.sinks < kMaxCount ? d.sinks : kMaxCount);
+    a.out_type = (uint32_t)d.out_type;
+    a.scale = (float)d.scale;
+    a.scale_log2 = (float)(d.scale * 1.4426950408889634);
+    a.status = device->d_status + bnn::kPagedStatusWord;
+    bnn::DeviceGuard guard(device->ordinal);
+    if (!guard.ok())
+        return BNN_EIO;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool wide = d.cache.head_dim == 128;
+    if (d.cache.type == BNN_PAGED_BF16)
+        return wide ? attention_typed<128, __nv_bfloat16>(a, s) : attention_typed<64, __nv_bfloat16>(a, s);
+    return wide ? attention_typed<128, __half>(a, s) : attention_typed<64, __half>(a, s);
+}
+
+BNN_Status bnn_b200_paged_sync(BNN_Device device, void* stream) {
+    if (!device)
+        return BNN_EINVAL;
+    bnn::DeviceGuard guard(device->ordinal);
+    if (!guard.ok())
+        return BNN_EIO;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int word = 0;
+    if (cudaMemcpyAsync(&word, device->d_status + bnn::kPagedStatusWord, sizeof(int), cudaMemcpyDeviceToHost, s) !=
+            cudaSuccess ||
+        cudaMemsetAsync(device->d_status + bnn::kPagedStatusWord, 0, sizeof(int), s) != cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess) {
+        cudaGetLastError();
+        return BNN_EIO;
+    }
+    if (word & bnn::kStatusTimeout)
+        return BNN_ETIMEOUT;
+    return word ? BNN_ERANGE : BNN_OK;
+}
+
+}  // extern "C"
