@@ -142,6 +142,7 @@ BNN_Status BNN_DeviceOpen(uint32_t device_index, BNN_Device* out_device) {
         return BNN_ENOMEM;
     d->ordinal = ordinal;
     bnn_noalloc_forget(ordinal);
+    bnn_paged_forget(ordinal);
     if (cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, ordinal) != cudaSuccess) {
         delete d;
         return BNN_EIO;

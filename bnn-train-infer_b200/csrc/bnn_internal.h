@@ -58,6 +58,8 @@ extern "C" BNN_Status bnn_b200_matrix_alloc(BNN_Device device, uint32_t in_featu
 // Drops the allocation-free GEMM's cached per-device set-up (bnn_noalloc.cu);
 // BNN_DeviceOpen calls it so a re-created device context is set up afresh.
 void bnn_noalloc_forget(int ordinal);
+// The same for the paged-cache kernels' shared-memory limits (paged.cu).
+void bnn_paged_forget(int ordinal);
 
 namespace bnn {
 

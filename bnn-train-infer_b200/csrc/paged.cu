@@ -1,11 +1,14 @@
 // paged.cu - host side of the paged-cache operators (include/bnn_b200_paged.h):
 // argument checks, the choice of kernel, launches.
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "bnn_b200_paged.h"
 #include "bnn_internal.h"
 #include "paged_append.cuh"
 #include "paged_common.cuh"
+#include "paged_decode.cuh"
 
 namespace {
 
@@ -95,7 +98,7 @@ BNN_Status append_source(const AppendArgs& a, int64_t type, bool interleaved, cu
 
 // The simple kernel: one warp per (token, query head).
 template <int D, typename T>
-static __global__ void __launch_bounds__(128) attention_rows_kernel(AttnArgs a) {
+static __global__ void __launch_bounds__(128) attention_rows_kernel(const __grid_constant__ AttnArgs a) {
     const uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 32;
     bnn::griddep_launch_dependents();
     bnn::griddep_wait();
@@ -112,7 +115,7 @@ static __global__ void __launch_bounds__(128) attention_rows_kernel(AttnArgs a) 
             hi = mid;
     }
     const Request r = load_request(a, lo);
-    if (t < r.start || t >= r.start + r.n)
+    if (t < r.start || t >= r.start + r.n || few_rows(a, r))
         return;
     if (r.n > (int32_t)a.max_q) {
         if ((threadIdx.x & 31) == 0)
@@ -122,8 +125,57 @@ static __global__ void __launch_bounds__(128) attention_rows_kernel(AttnArgs a) 
     attention_row<D, T>(a, lo, r, t - r.start, (uint32_t)(w % a.heads));
 }
 
+// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and
+// device. BNN_DeviceOpen forgets what was allowed (bnn_paged_forget).
+constexpr int kMaxDevices = 64, kMaxKernels = 16;
+std::mutex g_allowed_mutex;
+struct Allowed {
+    const void* kernel;
+    size_t bytes;
+} g_allowed[kMaxDevices][kMaxKernels];
+
+BNN_Status allow_smem(int ordinal, const void* kernel, size_t bytes) {
+    if (ordinal < 0 || ordinal >= kMaxDevices)
+        return BNN_ENOTSUP;
+    std::lock_guard<std::mutex> lock(g_allowed_mutex);
+    for (Allowed& e : g_allowed[ordinal]) {
+        if (e.kernel != nullptr && e.kernel != kernel)
+            continue;
+        if (e.kernel == kernel && e.bytes >= bytes)
+            return BNN_OK;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+            cudaGetLastError();
+            return BNN_EIO;
+        }
+        e = Allowed{kernel, bytes};
+        return BNN_OK;
+    }
+    return BNN_ENOTSUP;
+}
+
+// The workspace: two partial records for each CTA of the split kernel, then a
+// counter for each (request, KV head), zero between calls.
+uint32_t split_grid(BNN_Device device) { return (uint32_t)device->sm_count * kDecPerSm; }
+size_t partial_bytes(BNN_Device device) { return (size_t)split_grid(device) * 2 * DecodeShape<128>::kRecord * sizeof(float); }
+
 template <int D, typename T>
-BNN_Status attention_typed(const AttnArgs& a, cudaStream_t stream) {
+BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
+    const size_t smem = decode_smem(DecodeShape<D>::kRingBytes, a.batch);
+    const BNN_Status st = allow_smem(device->ordinal, (const void*)attention_split_kernel<D, T>, smem);
+    if (st != BNN_OK)
+        return st;
+    // no more CTAs than blocks there can be
+    const uint64_t per_row = (((uint64_t)a.table_width << a.c.page_shift) + kDecBlock - 1) / kDecBlock + 1;
+    const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * per_row;
+    return launch(attention_split_kernel<D, T>, dim3((uint32_t)std::min<uint64_t>(split_grid(device), most)), kDecThreads, smem,
+                  stream, a);
+}
+
+template <int D, typename T>
+BNN_Status attention_typed(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
+    const BNN_Status st = launch_split<D, T>(device, a, stream);
+    if (st != BNN_OK || (uint64_t)a.max_q * a.group <= kDecRows)
+        return st;
     const uint64_t blocks = ((uint64_t)a.tokens * a.heads + 3) / 4;
     if (blocks > INT32_MAX)
         return BNN_EINVAL;
@@ -131,6 +183,14 @@ BNN_Status attention_typed(const AttnArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+void bnn_paged_forget(int ordinal) {
+    if (ordinal < 0 || ordinal >= kMaxDevices)
+        return;
+    std::lock_guard<std::mutex> lock(g_allowed_mutex);
+    for (Allowed& e : g_allowed[ordinal])
+        e = Allowed{};
+}
 
 extern "C" {
 
@@ -198,7 +258,7 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
 BNN_Status bnn_b200_paged_workspace(BNN_Device device, int64_t batch, int64_t kv_heads, size_t* bytes) {
     if (!device || !bytes || batch <= 0 || batch > BNN_PAGED_MAX_BATCH || kv_heads <= 0 || kv_heads > 65536)
         return BNN_EINVAL;
-    *bytes = ((size_t)batch * (size_t)kv_heads * sizeof(int) + 255) & ~(size_t)255;
+    *bytes = partial_bytes(device) + (((size_t)batch * (size_t)kv_heads * sizeof(int) + 255) & ~(size_t)255);
     return BNN_OK;
 }
 
@@ -257,6 +317,8 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
     a.out_type = (uint32_t)d.out_type;
     a.scale = (float)d.scale;
     a.scale_log2 = (float)(d.scale * 1.4426950408889634);
+    a.partials = static_cast<float*>(d.workspace);
+    a.counters = reinterpret_cast<int*>(static_cast<unsigned char*>(d.workspace) + partial_bytes(device));
     a.status = device->d_status + bnn::kPagedStatusWord;
     bnn::DeviceGuard guard(device->ordinal);
     if (!guard.ok())
@@ -264,8 +326,8 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = d.cache.head_dim == 128;
     if (d.cache.type == BNN_PAGED_BF16)
-        return wide ? attention_typed<128, __nv_bfloat16>(a, s) : attention_typed<64, __nv_bfloat16>(a, s);
-    return wide ? attention_typed<128, __half>(a, s) : attention_typed<64, __half>(a, s);
+        return wide ? attention_typed<128, __nv_bfloat16>(device, a, s) : attention_typed<64, __nv_bfloat16>(device, a, s);
+    return wide ? attention_typed<128, __half>(device, a, s) : attention_typed<64, __half>(device, a, s);
 }
 
 BNN_Status bnn_b200_paged_sync(BNN_Device device, void* stream) {
