@@ -91,5 +91,6 @@ class DeviceGuard {
 // another unit's instance: bnn_b200_test_wait_limit sets every unit's copy.
 cudaError_t set_test_hooks_engine(unsigned long long limit_ns, int starve);
 cudaError_t set_test_hooks_noalloc(unsigned long long limit_ns, int starve);
+cudaError_t set_test_hooks_paged(unsigned long long limit_ns, int starve);
 
 }  // namespace bnn

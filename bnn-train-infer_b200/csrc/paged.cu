@@ -9,6 +9,7 @@
 #include "paged_append.cuh"
 #include "paged_common.cuh"
 #include "paged_decode.cuh"
+#include "paged_prefill.cuh"
 
 namespace {
 
@@ -96,35 +97,6 @@ BNN_Status append_source(const AppendArgs& a, int64_t type, bool interleaved, cu
 
 // ---- attention
 
-// The simple kernel: one warp per (token, query head).
-template <int D, typename T>
-static __global__ void __launch_bounds__(128) attention_rows_kernel(const __grid_constant__ AttnArgs a) {
-    const uint64_t w = (uint64_t)blockIdx.x * 4 + threadIdx.x / 32;
-    bnn::griddep_launch_dependents();
-    bnn::griddep_wait();
-    const int32_t t = (int32_t)(w / a.heads);
-    if (t >= (int32_t)a.tokens)
-        return;
-    // the last request that starts at or before t
-    uint32_t lo = 0, hi = a.batch;
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.q_starts[mid] <= t)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const Request r = load_request(a, lo);
-    if (t < r.start || t >= r.start + r.n || few_rows(a, r))
-        return;
-    if (r.n > (int32_t)a.max_q) {
-        if ((threadIdx.x & 31) == 0)
-            atomicOr(a.status, kPagedRange);
-        return;
-    }
-    attention_row<D, T>(a, lo, r, t - r.start, (uint32_t)(w % a.heads));
-}
-
 // Dynamic shared memory beyond 48 KB has to be allowed once per kernel and
 // device. BNN_DeviceOpen forgets what was allowed (bnn_paged_forget).
 constexpr int kMaxDevices = 64, kMaxKernels = 16;
@@ -171,18 +143,82 @@ BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t strea
                   stream, a);
 }
 
+// The tensor map of one pool: columns, rows of a page, heads, pages; a box is
+// 64 columns (the swizzle's 128 bytes) of up to 128 rows of one head's page.
+BNN_Status encode_map(CUtensorMap* map, const void* base, bool half, uint32_t d, const Cache& c, int64_t page, int64_t head,
+                      int64_t row) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<Encode>(fn);
+    }();
+    if (!encode)
+        return BNN_ENOTSUP;
+    const cuuint32_t rows = 1u << c.page_shift;
+    const cuuint64_t dims[4] = {d, rows, c.kv_heads, c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)page * 2};
+    const cuuint32_t box[4] = {64, std::min<cuuint32_t>(rows, kPfKeys), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult e = encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? BNN_OK : BNN_EIO;
+}
+
+template <int D, typename T, int kTiles>
+BNN_Status launch_tiles(BNN_Device device, const AttnArgs& a, cudaStream_t stream, bool every_request) {
+    using Shape = PrefillShape<D, kTiles>;
+    constexpr bool half = std::is_same<T, __half>::value;
+    PrefillArgs args;
+    args.a = a;
+    args.every_request = every_request;
+    BNN_Status st = encode_map(&args.k_map, a.c.k, half, D, a.c, a.c.k_page, a.c.k_head, a.c.k_row);
+    if (st == BNN_OK)
+        st = encode_map(&args.v_map, a.c.v, half, D, a.c, a.c.v_page, a.c.v_head, a.c.v_row);
+    if (st == BNN_OK)
+        st = allow_smem(device->ordinal, (const void*)attention_tiles_kernel<D, T, kTiles>, Shape::kSmem);
+    if (st != BNN_OK)
+        return st;
+    const uint64_t items = ((uint64_t)a.tokens * a.group) / (kTiles * kPfRows) + a.batch;  // at most
+    if (items * a.c.kv_heads > INT32_MAX)
+        return BNN_EINVAL;
+    return launch(attention_tiles_kernel<D, T, kTiles>, dim3((uint32_t)(items * a.c.kv_heads)), Shape::kThreads, Shape::kSmem,
+                  stream, args);
+}
+
 template <int D, typename T>
 BNN_Status attention_typed(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
-    const BNN_Status st = launch_split<D, T>(device, a, stream);
-    if (st != BNN_OK || (uint64_t)a.max_q * a.group <= kDecRows)
-        return st;
-    const uint64_t blocks = ((uint64_t)a.tokens * a.heads + 3) / 4;
-    if (blocks > INT32_MAX)
-        return BNN_EINVAL;
-    return launch(attention_rows_kernel<D, T>, dim3((uint32_t)blocks), 128, 0, stream, a);
+    // Requests of few rows go to the split kernel, the others to the tiles. One
+    // request is one kernel's, whatever its length.
+    if ((uint64_t)a.max_q * a.group <= kDecRows)
+        return launch_split<D, T>(device, a, stream);
+    const bool mixed = a.batch > 1;
+    if (mixed) {
+        const BNN_Status st = launch_split<D, T>(device, a, stream);
+        if (st != BNN_OK)
+            return st;
+    }
+    const uint64_t pairs = (((uint64_t)a.tokens * a.group) / (2 * kPfRows) + a.batch) * a.c.kv_heads;
+    return pairs >= (uint64_t)device->sm_count ? launch_tiles<D, T, 2>(device, a, stream, !mixed)
+                                               : launch_tiles<D, T, 1>(device, a, stream, !mixed);
 }
 
 }  // namespace
+
+namespace bnn {
+cudaError_t set_test_hooks_paged(unsigned long long limit_ns, int starve) {
+    cudaError_t e = cudaMemcpyToSymbol(g_wait_ns_limit, &limit_ns, sizeof limit_ns);
+    if (e == cudaSuccess)
+        e = cudaMemcpyToSymbol(paged::g_paged_starve, &starve, sizeof starve);
+    return e;
+}
+}  // namespace bnn
 
 void bnn_paged_forget(int ordinal) {
     if (ordinal < 0 || ordinal >= kMaxDevices)

@@ -1,0 +1,548 @@
+// paged_prefill.cuh - attention of prompt chunks over their pages on the
+// 5th-generation tensor cores.
+//
+// The group's query heads and a request's new tokens are the rows of one
+// matrix per KV head (row = token * group + head of the group), cut into
+// tiles of 128. For each tile of 128 keys
+//   S = Q K^T                     tcgen05.mma, both operands in shared memory
+//   P = 2^(c S - c m)             in registers, one thread per row
+//   O = O + P V                   tcgen05.mma, P from TMEM, V as it lies (MN-major)
+// with a running maximum m. m moves only when a row's maximum outgrows it by
+// more than 2^kSlack; then O (TMEM) and l are scaled by 2^(c (m_old - m_new)). The
+// result does not depend on m beyond rounding: weights reach at most 2^kSlack.
+//
+// A CTA holds kTiles tiles of 128 rows that share the K and V tiles: while the
+// tensor core multiplies for one, the other's threads take exponentials.
+// Warps: 4 per tile for the softmax (thread = row = TMEM lane), one that issues
+// the TMA loads, one that issues the products. K and V arrive page by page
+// (one box of up to 128 rows by 64 columns, 128-byte swizzle) in a ring of
+// 128-key tiles. A position that no row of the CTA sees may hold anything:
+// its scores are replaced, and its V row is overwritten with zeros before
+// the product.
+#pragma once
+
+#include <cuda.h>
+
+#include "paged_common.cuh"
+#include "paged_decode.cuh"
+#include "w1a8_mma.cuh"
+
+namespace bnn {
+namespace paged {
+
+constexpr uint32_t kPfKeys = 128;   // keys of a tile
+constexpr uint32_t kPfRows = 128;   // rows of a tile
+constexpr float kSlack = 8.0f;      // log2 of the largest weight
+
+template <int D, int kTiles>
+struct PrefillShape {
+    static constexpr uint32_t kThreads = kTiles * 128 + 64;
+    static constexpr uint32_t kTileBytes = kPfKeys * D * 2;  // of K, V or Q
+    static constexpr uint32_t kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 4 : 8);
+    static constexpr uint32_t kTmemUsed = kTiles * (kPfKeys + D);
+    static constexpr uint32_t kTmemCols = kTmemUsed <= 256 ? 256 : 512;
+    static constexpr uint32_t kBars = 2 * kStages + 3 * kTiles + 1;
+    static constexpr size_t kSmem = 1024 + (size_t)(kTiles + kStages) * kTileBytes + kBars * 8 + 16 * 4 + 64;
+};
+
+struct PrefillArgs {
+    AttnArgs a;
+    CUtensorMap k_map, v_map;
+    uint32_t every_request;  // 0: requests of few rows belong to the split kernel
+};
+
+// Test hook: a loader that issues nothing, so that every wait runs out.
+static __device__ int g_paged_starve = 0;
+
+// Instruction descriptor: D f32, A and B of one 16-bit type, M = 128; B K-major
+// (Q K^T) or MN-major (P V).
+template <typename T>
+__host__ __device__ constexpr uint32_t f16_idesc(uint32_t n, bool b_mn_major) {
+    const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// V's shared-memory descriptor: MN-major, 128-byte swizzle. Eight keys are
+// 1024 B apart (SBO); 64 columns on stand kPfKeys * 128 B further (LBO).
+__device__ __forceinline__ uint64_t mn_smem_desc(uint32_t saddr) {
+    const uint32_t lo = ((saddr >> 4) & 0x3fffu) | ((kPfKeys * 128u >> 4) << 16);
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+// 32 words to consecutive TMEM columns of this warp's lanes; complete after tmem_wait_st().
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+        : "memory");
+}
+
+// A box of `map` (64 columns from c0, rows from c1 of head c2 of page c3).
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t c1,
+                                            int32_t c2, int32_t c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Key tiles that rows of tokens at positions p0 .. p1 see.
+struct KeyTiles {
+    int32_t lo, sink_end, last;  // keys [0, sink_end) and [lo, last]
+    uint32_t sink_tiles, first, count;
+    __device__ __forceinline__ int32_t key(uint32_t t) const {
+        return (int32_t)((t < sink_tiles ? t : first + (t - sink_tiles)) * kPfKeys);
+    }
+};
+__device__ __forceinline__ KeyTiles key_tiles(const AttnArgs& a, int32_t p0, int32_t p1) {
+    KeyTiles k;
+    k.lo = window_begin(a, p0);
+    k.sink_end = (int32_t)min(a.sinks, (uint32_t)k.lo);
+    k.last = p1;
+    k.sink_tiles = ((uint32_t)k.sink_end + kPfKeys - 1) / kPfKeys;
+    k.first = max((uint32_t)k.lo / kPfKeys, k.sink_tiles);
+    const uint32_t end = p1 < 0 ? 0u : (uint32_t)p1 / kPfKeys + 1;
+    k.count = p1 < 0 ? 0u : k.sink_tiles + (end > k.first ? end - k.first : 0u);
+    return k;
+}
+
+template <int D, typename T, int kTiles>
+static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
+    attention_tiles_kernel(const __grid_constant__ PrefillArgs args) {
+    using Shape = PrefillShape<D, kTiles>;
+    constexpr uint32_t kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
+    constexpr uint32_t kHalves = D / 64;                // 64-column halves of a tile
+    constexpr uint32_t kHalfBytes = kPfKeys * 128;      // 16 KB
+    constexpr uint32_t kLoadWarp = kTiles * 4, kMmaWarp = kTiles * 4 + 1;
+    constexpr uint32_t kItemRows = kTiles * kPfRows;
+    const AttnArgs& a = args.a;
+    extern __shared__ __align__(1024) unsigned char pf_smem[];
+    const uint32_t raw = smem_addr(pf_smem);
+    unsigned char* sm = pf_smem + (((raw + 1023u) & ~1023u) - raw);
+    unsigned char* q_sm = sm;
+    unsigned char* ring = sm + kTiles * kTileBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kTileBytes);
+    uint64_t* empty = full + kStages;
+    uint64_t* q_ready = empty + kStages;     // [kTiles] Q in shared memory
+    uint64_t* s_ready = q_ready + kTiles;    // [kTiles] S in TMEM and the product before it done; at the end O complete
+    uint64_t* p_ready = s_ready + kTiles;    // [kTiles] P in TMEM, O scaled
+    uint64_t* drained = p_ready + kTiles;
+    uint32_t* mapped = reinterpret_cast<uint32_t*>(drained + 1);  // [16] bit u: 16-key part u of tile t (mod 16) is in memory
+    uint32_t* tmem_slot = mapped + 16;
+    __shared__ uint32_t warp_sum[32];
+    __shared__ uint32_t item_request, item_before;
+
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_launch_dependents();
+    if (tid == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int t = 0; t < kTiles; ++t) {
+            mbar_init(&q_ready[t], 4);
+            mbar_init(&s_ready[t], 1);
+            mbar_init(&p_ready[t], 4);
+        }
+        mbar_init(drained, 1);
+        fence_barrier_init();
+        item_request = ~0u;
+    }
+    griddep_wait();
+
+    // ---- which rows: items of kItemRows rows, request by request, heads side by
+    // side; the last ones (they see the most keys of a prompt) first
+    uint32_t total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        const uint32_t mine = total;  // pass 1: the number of items
+        uint32_t seen = 0;
+        for (uint32_t b0 = 0; b0 < a.batch; b0 += Shape::kThreads) {
+            const uint32_t b = b0 + tid;
+            uint32_t x = 0;
+            if (b < a.batch) {
+                const Request r = load_request(a, b);
+                if (r.n > (int32_t)a.max_q) {
+                    if (blockIdx.x == 0)
+                        atomicOr(a.status, kPagedRange);
+                } else if (r.n > 0 && (args.every_request || !few_rows(a, r))) {
+                    x = ((uint32_t)r.n * a.group + kItemRows - 1) / kItemRows;
+                }
+            }
+            uint32_t sum = x;
+#pragma unroll
+            for (uint32_t d = 1; d < 32; d <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
+                sum += lane >= d ? y : 0;
+            }
+            if (lane == 31)
+                warp_sum[warp] = sum;
+            __syncthreads();
+            uint32_t before = seen;
+            for (uint32_t w = 0; w < Shape::kThreads / 32; ++w) {
+                before += w < warp ? warp_sum[w] : 0;
+                seen += warp_sum[w];
+            }
+            if (pass == 1) {
+                const uint32_t item = mine - 1 - blockIdx.x / a.c.kv_heads;
+                const uint32_t at = before + sum - x;
+                if (item >= at && item < at + x) {
+                    item_request = b;
+                    item_before = at;
+                }
+            }
+            __syncthreads();
+        }
+        total = seen;
+        if (pass == 0 && blockIdx.x / a.c.kv_heads >= total)
+            return;
+    }
+    const uint32_t b = item_request, kvh = blockIdx.x % a.c.kv_heads;
+    const Request r = load_request(a, b);
+    const uint32_t row0 = (total - 1 - blockIdx.x / a.c.kv_heads - item_before) * kItemRows;
+    const uint32_t rows = (uint32_t)r.n * a.group;
+    const int32_t base_pos = r.kv - r.n;
+    const KeyTiles tiles = key_tiles(a, base_pos + (int32_t)(row0 / a.group),
+                                     base_pos + (int32_t)(min(row0 + kItemRows, rows) - 1) / (int32_t)a.group);
+    const uint32_t count = tiles.count;
+
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                     "r"(Shape::kTmemCols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem_o = tmem + kTiles * kPfKeys;
+
+    if (warp == kLoadWarp) {
+        // ---- K and V tiles, page by page: lane p has the tile's p-th page
+        const uint32_t page_rows = min(1u << a.c.page_shift, kPfKeys);
+        const uint32_t per_tile = kPfKeys / page_rows;
+        uint32_t slot = 0, round = 0;
+        const bool starved = *reinterpret_cast<volatile int*>(&g_paged_starve) != 0;
+        for (uint32_t t = 0; t < count; ++t) {
+            const int32_t j = tiles.key(t) + (int32_t)(lane * page_rows);
+            const bool need = lane < per_tile && j <= tiles.last && (j + (int32_t)page_rows > tiles.lo || j < tiles.sink_end);
+            const int32_t page = need ? page_of(a, b, j) : -1;
+            const uint32_t parts = page_rows / 16;
+            const uint32_t bits =
+                __reduce_or_sync(0xffffffffu, page >= 0 ? ((1u << parts) - 1u) << (lane * parts) : 0u);
+            const uint32_t bytes = (uint32_t)__popc(bits) * 16 * D * 2;
+            const int32_t in_page = j & ((1 << a.c.page_shift) - 1);
+            bool ok = true;
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                if (round > 0)
+                    ok = mbar_wait(&empty[slot], (round - 1) & 1);
+                if (!ok || starved)
+                    break;
+                if (lane == 0) {
+                    if (which == 0)
+                        mapped[t % 16] = bits;
+                    mbar_arrive_expect_tx(&full[slot], bytes);
+                }
+                __syncwarp();
+                if (page >= 0) {
+                    const uint32_t dst = smem_addr(ring + slot * kTileBytes) + lane * page_rows * 128;
+#pragma unroll
+                    for (uint32_t h = 0; h < kHalves; ++h)
+                        tma_load_4d(dst + h * kHalfBytes, which ? &args.v_map : &args.k_map, &full[slot], (int32_t)(h * 64),
+                                    in_page, (int32_t)kvh, page);
+                }
+                __syncwarp();
+                if (++slot == kStages) {
+                    slot = 0;
+                    ++round;
+                }
+            }
+            if (!ok || starved) {
+                if (lane == 0)
+                    atomicOr(a.status, kStatusTimeout);
+                break;
+            }
+        }
+        // no copy may be in flight when the CTA exits
+        const uint32_t issued = round * kStages + slot;
+        for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+            if (!mbar_wait(&full[i % kStages], (i / kStages) & 1) && lane == 0)
+                atomicOr(a.status, kStatusTimeout);
+    } else if (warp == kMmaWarp) {
+        // ---- the products; tile by tile Q K^T of the next keys right after P V
+        constexpr uint32_t kQkDesc = f16_idesc<T>(kPfKeys, false), kPvDesc = f16_idesc<T>(D, true);
+        bool ok = true;
+        auto need = [&](uint64_t* bar, uint32_t parity) {
+            ok = ok && mbar_wait(bar, parity);
+            return ok;
+        };
+        auto slot_of = [&](uint32_t t, uint32_t which) { return (2 * t + which) % kStages; };
+        auto parity_of = [&](uint32_t t, uint32_t which) { return ((2 * t + which) / kStages) & 1; };
+        auto qk = [&](uint32_t tile, uint32_t t) {
+            if (lane == 0) {
+                const uint32_t qa = smem_addr(q_sm) + tile * kTileBytes;
+                const uint32_t ka = smem_addr(ring) + slot_of(t, 0) * kTileBytes;
+#pragma unroll
+                for (uint32_t k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k / 4) * kHalfBytes + (k % 4) * 32;
+                    mma_f16_ss(tmem + tile * kPfKeys, mma_smem_desc(qa + off), mma_smem_desc(ka + off), kQkDesc, k != 0);
+                }
+            }
+        };
+        auto pv = [&](uint32_t tile, uint32_t t) {
+            if (lane == 0) {
+                const uint32_t va = smem_addr(ring) + slot_of(t, 1) * kTileBytes;
+#pragma unroll
+                for (uint32_t k = 0; k < kPfKeys / 16; ++k)
+                    mma_f16_ts(tmem_o + tile * D, tmem + tile * kPfKeys + k * 8, mn_smem_desc(va + k * 16 * 128), kPvDesc,
+                               t != 0 || k != 0);
+            }
+        };
+        auto commit = [&](uint64_t* bar) {
+            if (lane == 0)
+                mma_commit(bar);
+        };
+        if (count > 0 && need(&full[slot_of(0, 0)], 0)) {
+#pragma unroll
+            for (uint32_t tile = 0; tile < kTiles; ++tile) {
+                if (!need(&q_ready[tile], 0))
+                    break;
+                tc_fence_after();
+                qk(tile, 0);
+                commit(&s_ready[tile]);
+            }
+            commit(&empty[slot_of(0, 0)]);
+            for (uint32_t t = 0; ok && t < count; ++t) {
+                if (!need(&full[slot_of(t, 1)], parity_of(t, 1)))
+                    break;
+                // V rows that no row of this CTA sees: zeros
+                const int32_t key0 = tiles.key(t);
+                const uint32_t bits = mapped[t % 16];
+                if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > tiles.last || key0 < tiles.lo) {
+                    unsigned char* v = ring + slot_of(t, 1) * kTileBytes;
+                    for (uint32_t row = lane / 8; row < kPfKeys; row += 4) {
+                        const int32_t j = key0 + (int32_t)row;
+                        const bool used = (bits >> (row / 16) & 1u) && j <= tiles.last && (j >= tiles.lo || j < tiles.sink_end);
+                        if (!used)
+#pragma unroll
+                            for (uint32_t h = 0; h < kHalves; ++h)
+                                *reinterpret_cast<uint4*>(v + h * kHalfBytes + row * 128 + (lane % 8) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                if (t + 1 < count && !need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0)))
+                    break;
+#pragma unroll
+                for (uint32_t tile = 0; tile < kTiles; ++tile) {
+                    if (!need(&p_ready[tile], t & 1))
+                        break;
+                    tc_fence_after();
+                    pv(tile, t);
+                    if (tile == kTiles - 1)
+                        commit(&empty[slot_of(t, 1)]);
+                    if (t + 1 < count) {
+                        qk(tile, t + 1);
+                        if (tile == kTiles - 1)
+                            commit(&empty[slot_of(t + 1, 0)]);
+                    }
+                    commit(&s_ready[tile]);
+                }
+            }
+            if (!ok && lane == 0)
+                atomicOr(a.status, kStatusTimeout);
+        } else if (!ok && lane == 0) {
+            atomicOr(a.status, kStatusTimeout);
+        }
+        // the TMEM may go when every product issued has completed
+        commit(drained);
+        if (!mbar_wait(drained, 0) && lane == 0)
+            atomicOr(a.status, kStatusTimeout);
+    } else {
+        // ---- softmax: thread = row
+        const uint32_t tile = warp / 4, wrow = row0 + tile * kPfRows + (warp % 4) * 32;  // the warp's first row
+        const uint32_t lane_off = ((warp % 4) * 32u) << 16;
+        const uint32_t t_s = tmem + tile * kPfKeys + lane_off, t_o = tmem_o + tile * D + lane_off;
+        {
+            unsigned char* q = q_sm + tile * kTileBytes;
+            constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
+#pragma unroll 4
+            for (uint32_t i = 0; i < 32 / kAtOnce; ++i) {
+                const uint32_t in_warp = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                const uint32_t row = wrow + in_warp, tr = (warp % 4) * 32 + in_warp;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (row < rows) {
+                    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + (int32_t)(row / a.group)) * a.q_token +
+                                 (int64_t)(kvh * a.group + row % a.group) * a.q_head + chunk * 8;
+                    if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0)
+                        w = *reinterpret_cast<const uint4*>(p);
+                    else
+                        w = make_uint4(load_pair<T>(p), load_pair<T>(p + 2), load_pair<T>(p + 4), load_pair<T>(p + 6));
+                }
+                *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&q_ready[tile]);
+        }
+        const uint32_t my_row = wrow + lane;
+        const int32_t token = (int32_t)min(my_row / a.group, (uint32_t)r.n - 1);
+        const int32_t pos = base_pos + token, lo = window_begin(a, pos);
+        const int32_t first_pos = base_pos + (int32_t)min(wrow / a.group, (uint32_t)r.n - 1);
+        const int32_t last_lo = window_begin(a, base_pos + (int32_t)min((wrow + 31) / a.group, (uint32_t)r.n - 1));
+        const float c = a.scale_log2;
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        uint32_t t = 0;
+        for (; t < count; ++t) {
+            if (!(ok = mbar_wait(&s_ready[tile], t & 1)))
+                break;
+            tc_fence_after();
+            uint32_t s[kPfKeys];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+                tmem_ld32(t_s + i * 32, s + i * 32);
+            tmem_wait();
+            const int32_t key0 = tiles.key(t);
+            const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
+            if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
+                const int32_t hi = pos - key0, low = lo - key0, sink = (int32_t)a.sinks - key0;
+#pragma unroll
+                for (int32_t i = 0; i < (int32_t)kPfKeys; ++i) {
+                    const bool seen = i <= hi && (i >= low || i < sink) && (bits >> (i / 16) & 1u);
+                    s[i] = seen ? s[i] : 0xff800000u;
+                }
+            }
+            float mx[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                mx[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
+#pragma unroll
+            for (int i = 8; i < (int)kPfKeys; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx[e] = max3(mx[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            const bool grow = top > m && (top - m) * c > kSlack;  // also the first finite score
+            if (__any_sync(0xffffffffu, grow)) {
+                const float mn = grow ? top : m;
+                const float w = grow ? exp2_fast((m - mn) * c) : 1.0f;
+                if (t > 0) {
+                    // the product of the last keys has completed (s_ready)
+#pragma unroll
+                    for (uint32_t i = 0; i < D / 32; ++i) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + i * 32, o);
+                        tmem_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * w);
+                        tmem_st32(t_o + i * 32, o);
+                    }
+                }
+                l *= w;
+                m = mn;
+            }
+            const float neg = m == -INFINITY ? 0.0f : -m * c;
+            const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(neg, neg);
+            uint64_t sum2[2] = {0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < kPfKeys; i += 64) {
+                uint32_t p[32];
+#pragma unroll
+                for (uint32_t e = 0; e < 64; e += 2) {
+                    const uint64_t y = f2_fma((uint64_t)s[i + e] | ((uint64_t)s[i + e + 1] << 32), c2, n2);
+                    const float lo_p = exp2_fast(f2_lo(y)), hi_p = exp2_fast(f2_hi(y));
+                    sum2[(e / 2) & 1] = f2_add(sum2[(e / 2) & 1], f2_pack(lo_p, hi_p));
+                    p[e / 2] = pack2<T>(lo_p, hi_p);
+                }
+                tmem_st32(t_s + i / 2, p);
+            }
+            l += (f2_lo(sum2[0]) + f2_hi(sum2[0])) + (f2_lo(sum2[1]) + f2_hi(sum2[1]));
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(&p_ready[tile]);
+        }
+        if (ok && count > 0)
+            ok = mbar_wait(&s_ready[tile], count & 1);
+        if (!ok && lane == 0)
+            atomicOr(a.status, kStatusTimeout);
+        if (ok) {
+            tc_fence_after();
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const uint32_t head = kvh * a.group + my_row % a.group;
+            const int64_t tok = r.start + (int64_t)(my_row / a.group);
+            const int64_t at = tok * a.o_token + (int64_t)head * a.o_head;
+            bool odd = false;
+#pragma unroll
+            for (uint32_t i = 0; i < D / 32; ++i) {
+                uint32_t o[32];
+                if (count > 0) {
+                    tmem_ld32(t_o + i * 32, o);
+                    tmem_wait();
+                }
+                if (my_row < rows)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float x[4];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) {
+                            x[f] = l == 0.0f ? 0.0f : __uint_as_float(o[e + f]) * inv;
+                            odd |= !finite32(x[f]);
+                        }
+                        store_out4<T>(a, at + i * 32 + e, x);
+                    }
+            }
+            if (a.lse && my_row < rows)
+                a.lse[tok * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, logf(l));
+            // a row that came out infinite or NaN may owe it to a value that
+            // only later tokens see: again, key by key
+            uint32_t again = __ballot_sync(0xffffffffu, odd);
+            while (again) {
+                const uint32_t i = (uint32_t)__ffs((int)again) - 1;
+                again &= again - 1;
+                attention_row<D, T>(a, b, r, (int32_t)((wrow + i) / a.group), kvh * a.group + (wrow + i) % a.group);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Shape::kTmemCols));
+    }
+}
+
+}  // namespace paged
+}  // namespace bnn

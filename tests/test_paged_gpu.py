@@ -525,3 +525,25 @@ def test_append_refusals(ops):
     refused(ENOTSUP, q[..., :32], k[..., :32], v[..., :32], cos[:, :16].contiguous(), sin[:, :16].contiguous(), p, s, kp[..., :32],
             vp[..., :32])
     ops.sync()
+
+
+def test_starved_loads_time_out_then_recover(ops):
+    """With the tiles kernel's loads withheld and the limit at 1 ms every wait of it runs
+    out (nothing faults, nothing is in flight); the next sync says so, and with the limits
+    restored the same call is right."""
+    import ctypes
+    from bnn_b200 import accel
+    hook = ops.device.api.dll.bnn_b200_test_wait_limit
+    hook.restype, hook.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int]
+    made = make([(200, 300), (40, 40)], 4, 2, 128, 16, BF16)
+    torch.cuda.synchronize()
+    assert hook(ops.device.handle, 1_000_000, 1) == accel.OK
+    try:
+        ops.attention(*made, max_q=200)
+        with pytest.raises(accel.BnnError) as e:
+            ops.sync()
+    finally:
+        torch.cuda.synchronize()
+        assert hook(ops.device.handle, 0, 0) == accel.OK
+    assert e.value.status == accel.ETIMEOUT
+    check(ops, made)
