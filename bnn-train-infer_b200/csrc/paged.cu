@@ -125,10 +125,11 @@ BNN_Status allow_smem(int ordinal, const void* kernel, size_t bytes) {
     return BNN_ENOTSUP;
 }
 
-// The workspace: two partial records for each CTA of the split kernel, then a
-// counter for each (request, KV head), zero between calls.
+// The workspace: for each CTA of the split kernel two records of partial rows
+// and two of joined groups; then two counters for each CTA and one for each
+// (request, KV head), zero between calls.
 uint32_t split_grid(BNN_Device device) { return (uint32_t)device->sm_count * kDecPerSm; }
-size_t partial_bytes(BNN_Device device) { return (size_t)split_grid(device) * 2 * DecodeShape<128>::kRecord * sizeof(float); }
+size_t partial_bytes(BNN_Device device) { return (size_t)split_grid(device) * 4 * DecodeShape<128>::kRecord * sizeof(float); }
 
 template <int D, typename T>
 BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
@@ -139,6 +140,8 @@ BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t strea
     // no more CTAs than blocks there can be
     const uint64_t per_row = (((uint64_t)a.table_width << a.c.page_shift) + kDecBlock - 1) / kDecBlock + 1;
     const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * per_row;
+    if (most > INT32_MAX)
+        return BNN_ENOTSUP;  // blocks are counted in 32 bits
     return launch(attention_split_kernel<D, T>, dim3((uint32_t)std::min<uint64_t>(split_grid(device), most)), kDecThreads, smem,
                   stream, a);
 }
@@ -294,7 +297,7 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
 BNN_Status bnn_b200_paged_workspace(BNN_Device device, int64_t batch, int64_t kv_heads, size_t* bytes) {
     if (!device || !bytes || batch <= 0 || batch > BNN_PAGED_MAX_BATCH || kv_heads <= 0 || kv_heads > 65536)
         return BNN_EINVAL;
-    *bytes = partial_bytes(device) + (((size_t)batch * (size_t)kv_heads * sizeof(int) + 255) & ~(size_t)255);
+    *bytes = partial_bytes(device) + (((2 * (size_t)split_grid(device) + (size_t)batch * (size_t)kv_heads) * sizeof(int) + 255) & ~(size_t)255);
     return BNN_OK;
 }
 
@@ -354,7 +357,8 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
     a.scale = (float)d.scale;
     a.scale_log2 = (float)(d.scale * 1.4426950408889634);
     a.partials = static_cast<float*>(d.workspace);
-    a.counters = reinterpret_cast<int*>(static_cast<unsigned char*>(d.workspace) + partial_bytes(device));
+    a.group_counters = reinterpret_cast<int*>(static_cast<unsigned char*>(d.workspace) + partial_bytes(device));
+    a.row_counters = a.group_counters + 2 * split_grid(device);
     a.status = device->d_status + bnn::kPagedStatusWord;
     bnn::DeviceGuard guard(device->ordinal);
     if (!guard.ok())

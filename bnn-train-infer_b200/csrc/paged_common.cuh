@@ -39,8 +39,9 @@ struct AttnArgs {
     uint32_t out_type;
     float scale;       // score scale
     float scale_log2;  // scale * log2(e)
-    float* partials;   // workspace of the split kernel
-    int* counters;
+    float* partials;   // workspace of the split kernel: records of partial rows
+    int* group_counters;
+    int* row_counters;
     int* status;
 };
 
@@ -107,8 +108,7 @@ __device__ __forceinline__ Request load_request(const AttnArgs& a, uint32_t b) {
     const int32_t tokens = (int32_t)a.tokens;
     r.start = min(max(a.q_starts[b], 0), tokens);
     r.n = max(min(a.q_starts[b + 1], tokens) - r.start, 0);
-    const int64_t room = min((int64_t)a.table_width << a.c.page_shift, (int64_t)1 << 30);
-    r.kv = (int32_t)min((int64_t)max(a.kv_lens[b], 0), room);
+    r.kv = min(max(a.kv_lens[b], 0), (int32_t)min((uint64_t)a.table_width << a.c.page_shift, (uint64_t)1 << 30));
     return r;
 }
 
@@ -131,6 +131,21 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, float x
         const uint32_t w = pack2<T>(x, 0.0f);
         reinterpret_cast<uint16_t*>(a.out)[at] = (uint16_t)w;
     }
+}
+
+// ln(x) for a softmax sum (one MUFU operation: off by 2^-22 at most for x near
+// one, relatively elsewhere).
+__device__ __forceinline__ float ln_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y * 0.693147182f;
+}
+
+// mbar_wait (bnn_sync.cuh) with the waiting itself out of line: these kernels
+// wait at many places, and a call of few tiles runs each once.
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+    return mbar_try_wait(bar, parity) || wait_slow(bar, parity);
 }
 
 // The whole of one output row by one warp, straight from the definition: a
@@ -190,7 +205,7 @@ __device__ __noinline__ void attention_row(const AttnArgs& a, uint32_t b, const 
     for (int e = 0; e < E; ++e)
         store_out<T>(a, at + e, l == 0.0f ? 0.0f : o[e] / l);
     if (a.lse && lane == 0)
-        a.lse[(int64_t)(r.start + i) * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, logf(l));
+        a.lse[(int64_t)(r.start + i) * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, ln_fast(l));
 }
 
 }  // namespace paged

@@ -13,7 +13,10 @@
 // a row that falls into several shares is joined by the CTA that finishes it
 // last, in the order of the shares (the result does not depend on timing), and
 // rows of at most kWholeBlocks blocks are not cut. Each warp streams its own
-// 16-key tiles through a ring of cp.async stages: no CTA barrier inside a row.
+// 16-key tiles through a ring of cp.async stages, across the rows of its share:
+// the next row's tiles are on their way while the warps' parts of this one are
+// joined. The code is kept small on purpose: a short call runs most of it
+// once, and its instructions come from memory.
 #pragma once
 
 #include <type_traits>
@@ -31,6 +34,7 @@ constexpr uint32_t kDecPerSm = 2;                        // CTAs an SM holds
 constexpr uint32_t kWholeBlocks = 8;
 constexpr uint32_t kMinShare = 4;                        // blocks
 constexpr uint32_t kDecRows = 16;
+constexpr uint32_t kJoin = 16;                           // parts of a row that one CTA joins at a time
 
 template <int D>
 struct DecodeShape {
@@ -42,7 +46,7 @@ struct DecodeShape {
     static_assert(kDecRows * D * 4 <= kWarpBytes, "a warp's O fits its ring");
 };
 
-inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * 8 + 16; }
+inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * 4 + 16; }
 
 // The 64-key blocks of a request that some of its new tokens see: the sinks'
 // blocks, then those from the first token's window on.
@@ -110,26 +114,48 @@ __device__ __forceinline__ uint32_t load_pair(const T* p) {
     return (uint32_t)h[0] | ((uint32_t)h[1] << 16);
 }
 
-// Four adjacent result values, one store where the address allows it.
+// Four adjacent result values at any alignment and of either type.
+template <typename T>
+__device__ __noinline__ void store_out4_any(const AttnArgs& a, int64_t at, float x0, float x1, float x2, float x3) {
+    store_out<T>(a, at, x0);
+    store_out<T>(a, at + 1, x1);
+    store_out<T>(a, at + 2, x2);
+    store_out<T>(a, at + 3, x3);
+}
 template <typename T>
 __device__ __forceinline__ void store_out4(const AttnArgs& a, int64_t at, const float (&x)[4]) {
-    if (a.out_type == kTypeF32) {
-        float* p = reinterpret_cast<float*>(a.out) + at;
-        if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-            *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-            return;
-        }
-    } else {
-        uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + at;
-        if ((reinterpret_cast<uintptr_t>(p) & 7u) == 0) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
-            return;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        store_out<T>(a, at + e, x[e]);
+    uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + at;
+    if (a.out_type != kTypeF32 && (reinterpret_cast<uintptr_t>(p) & 7u) == 0)
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+    else
+        store_out4_any<T>(a, at, x[0], x[1], x[2], x[3]);
 }
+
+// Scales and writes four values of one output row (and its lse with d == 0);
+// notes a row that is not finite.
+template <typename T>
+__device__ __noinline__ void finish4(const AttnArgs& a, uint32_t tok, uint32_t head, uint32_t d, float4 p, float sum, float mm,
+                                     uint32_t* odd_rows, uint32_t row) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float v[4] = {p.x * inv, p.y * inv, p.z * inv, p.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = sum == 0.0f ? 0.0f : v[e];
+        if (!finite32(v[e]))
+            atomicOr(odd_rows, 1u << row);
+    }
+    store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
+    if (a.lse && d == 0)
+        a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, ln_fast(sum));
+}
+
+// One stretch of a share: blocks [y0, y1) of row (b, kvh), which spans blocks
+// [row_begin, row_begin + sp.count) of the call.
+struct Segment {
+    Request r;
+    Span sp;
+    uint32_t b, kvh, row_begin, y0, y1;
+};
 
 template <int D, typename T>
 static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split_kernel(const __grid_constant__ AttnArgs a) {
@@ -137,8 +163,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     constexpr uint32_t kStages = Shape::kStages, kStage = Shape::kStageBytes;
     constexpr uint32_t kChunks = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) unsigned char smem[];
-    uint64_t* prefix = reinterpret_cast<uint64_t*>(smem + Shape::kRingBytes);  // [batch + 1] blocks before a request
-    __shared__ uint64_t warp_sum[kDecWarps];
+    uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + Shape::kRingBytes);  // [batch + 1] blocks before a request
+    __shared__ uint32_t warp_sum[kDecWarps];
     __shared__ float joint_m[kDecWarps][kDecRows], joint_l[kDecWarps][kDecRows];
     __shared__ uint32_t odd_rows;
     __shared__ int last_arriver;
@@ -149,26 +175,27 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     griddep_wait();
 
     // ---- blocks of every request, and this CTA's share of them
-    uint64_t total = 0;
+    uint32_t total = 0;
+#pragma unroll 1
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kDecThreads) {
         const uint32_t b = b0 + tid;
-        uint64_t x = 0;
+        uint32_t x = 0;
         if (b < a.batch) {
             const Request r = load_request(a, b);
             if (r.n > (int32_t)a.max_q && blockIdx.x == 0)
                 atomicOr(a.status, kPagedRange);
-            x = few_rows(a, r) ? (uint64_t)span_of(a, r).count * a.c.kv_heads : 0;
+            x = few_rows(a, r) ? span_of(a, r).count * a.c.kv_heads : 0;
         }
-        uint64_t sum = x;
+        uint32_t sum = x;
 #pragma unroll
         for (uint32_t d = 1; d < 32; d <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, sum, d);
+            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
             sum += lane >= d ? y : 0;
         }
         if (lane == 31)
             warp_sum[warp] = sum;
         __syncthreads();
-        uint64_t before = total;
+        uint32_t before = total;
 #pragma unroll
         for (uint32_t w = 0; w < kDecWarps; ++w) {
             before += w < warp ? warp_sum[w] : 0;
@@ -178,17 +205,23 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             prefix[b] = before + sum - x;
         __syncthreads();
     }
-    if (tid == 0)
+    if (tid == 0) {
         prefix[a.batch] = total;
+        odd_rows = 0;
+    }
     __syncthreads();
-    const uint64_t rows = (uint64_t)a.batch * a.c.kv_heads;
-    const uint64_t shares = min((uint64_t)gridDim.x, max((total + kMinShare - 1) / kMinShare, min(rows, total)));
+    if (total == 0)
+        return;
+    const uint32_t rows = a.batch * a.c.kv_heads;
+    const uint32_t shares = min(gridDim.x, max((total + kMinShare - 1) / kMinShare, min(rows, total)));
     if (blockIdx.x >= shares)
         return;
+    const uint32_t even = total / shares, extra = total % shares;  // the first `extra` shares have one block more
 
     // the request that block x belongs to
-    auto request_at = [&](uint64_t x) {
+    auto request_at = [&](uint32_t x) {
         uint32_t lo = 0, hi = a.batch;
+#pragma unroll 1
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
             if (prefix[mid] <= x)
@@ -198,47 +231,128 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         }
         return lo;
     };
-    // first block of share c: inside a short row it moves to the row's start
-    auto share_begin = [&](uint64_t c) {
-        const uint64_t x = c * total / shares;
-        if (c == 0 || c >= shares)
-            return x;
-        const uint32_t b = request_at(x);
-        const uint64_t len = (prefix[b + 1] - prefix[b]) / a.c.kv_heads;
-        return len > kWholeBlocks ? x : x - (x - prefix[b]) % len;
+    // first block of share c; inside a short row it moves to the row's start
+    auto raw_begin = [&](uint32_t c) { return c * even + min(c, extra); };
+    uint32_t ends[2];
+#pragma unroll 1
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t at = raw_begin(blockIdx.x + i);
+        uint32_t begin = at;
+        if (at < total) {
+            const uint32_t b = request_at(at), len = (prefix[b + 1] - prefix[b]) / a.c.kv_heads;
+            begin = len > kWholeBlocks ? at : at - (at - prefix[b]) % len;
+        }
+        ends[0] = i == 0 ? begin : ends[0];
+        ends[1] = begin;
+    }
+    const uint32_t x_begin = ends[0], x_end = ends[1];
+    if (x_begin >= x_end)
+        return;
+    auto segment_at = [&](uint32_t x) {
+        Segment s;
+        s.b = request_at(x);
+        s.r = load_request(a, s.b);
+        s.sp = span_of(a, s.r);
+        const uint32_t in = x - prefix[s.b];
+        s.kvh = in / s.sp.count;
+        s.y0 = in - s.kvh * s.sp.count;
+        s.row_begin = x - s.y0;
+        s.y1 = min(x_end - s.row_begin, s.sp.count);
+        return s;
     };
-    uint64_t x = share_begin(blockIdx.x);
-    const uint64_t x_end = share_begin(blockIdx.x + 1);
 
-    unsigned char* ring = smem + warp * Shape::kWarpBytes;
-    const uint32_t ring_addr = smem_addr(ring);
-    bool first_segment = true;
+    const uint32_t ring_addr = smem_addr(smem) + warp * Shape::kWarpBytes;
+    const uint32_t page_mask = (1u << a.c.page_shift) - 1u;
+    auto tile_key = [&](const Segment& s, uint32_t y) { return s.sp.key(y) + (int32_t)(warp * kDecTile); };
 
+    // ---- what is fetched: the next tile is block fy of segment f; the lanes
+    // hold the pages of its 32 blocks from `base` on, and of the 32 after them
+    Segment f = segment_at(x_begin);
+    uint32_t fx = x_begin, fy = f.y0, base = fy, slot_f = 0;
+    auto lookup = [&](uint32_t y) -> int32_t {
+        if (y >= f.y1)
+            return -1;
+        const int32_t j = tile_key(f, y);
+        return j < f.r.kv ? page_of(a, f.b, j) : -1;
+    };
+    int32_t pages = lookup(base + lane), more = -1;
+    uint32_t valid = 0, in_flight = 0;  // bit i: the i-th tile in flight lies in a page
+    // rows that no token sees arrive as zeros: whatever the cache holds
+    // there (a weight of zero times NaN is NaN) stays out of the product
+    auto fetch = [&]() {
+        if (fx < x_end) {
+            const int32_t page = __shfl_sync(0xffffffffu, pages, (int)(fy - base));
+            const int32_t j0 = tile_key(f, fy);
+            const uint32_t at = ring_addr + slot_f * kStage;
+            const int64_t head = (int64_t)f.kvh, in_page = (int64_t)((uint32_t)j0 & page_mask);
+            const T* kp = reinterpret_cast<const T*>(a.c.k);
+            const T* vp = reinterpret_cast<const T*>(a.c.v);
+            if (page >= 0) {
+                kp += head * a.c.k_head + (int64_t)page * a.c.k_page + in_page * a.c.k_row;
+                vp += head * a.c.v_head + (int64_t)page * a.c.v_page + in_page * a.c.v_row;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kDecTile * kChunks / 32; ++i) {
+                const uint32_t row = i * (32 / kChunks) + lane / kChunks, chunk = lane % kChunks;
+                const int32_t j = j0 + (int32_t)row;
+                const bool take = page >= 0 && j < f.r.kv && (j >= f.sp.lo || j < f.sp.sink_end);
+                const uint32_t dst = at + row * (D * 2) + ((chunk ^ (row & 7u)) * 16u);
+                copy16(dst, kp + (take ? (int64_t)row * a.c.k_row + chunk * 8 : 0), take);
+                copy16(dst + kDecTile * D * 2, vp + (take ? (int64_t)row * a.c.v_row + chunk * 8 : 0), take);
+            }
+            valid |= (page >= 0 ? 1u : 0u) << in_flight;
+            ++in_flight;
+            slot_f = slot_f + 1 == kStages ? 0 : slot_f + 1;
+            ++fx;
+            ++fy;
+            if (fy == f.y1) {
+                if (fx < x_end) {
+                    f = segment_at(fx);
+                    fy = base = f.y0;
+                    pages = lookup(base + lane);
+                }
+            } else if (fy - base == 32) {
+                base = fy;
+                pages = more;
+            } else if (fy - base == 8) {
+                more = lookup(base + 32 + lane);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (uint32_t s = 0; s < kStages - 1; ++s)
+        fetch();
+
+    uint32_t x = x_begin, slot = 0;
     while (x < x_end) {
-        // ---- one segment: blocks [y0, y1) of row (b, kvh)
-        const uint32_t b = request_at(x);
-        const Request r = load_request(a, b);
-        const Span sp = span_of(a, r);
-        const uint64_t in = x - prefix[b];
-        const uint32_t kvh = (uint32_t)(in / sp.count), y0 = (uint32_t)(in % sp.count);
-        const uint64_t row_begin = x - y0, row_end = row_begin + sp.count;
-        const uint32_t y1 = (uint32_t)(min(x_end, row_end) - row_begin);
-        const uint32_t nrows = (uint32_t)r.n * a.group;
-
+        // ---- one segment
+        const Segment s = segment_at(x);
+        const uint32_t nrows = (uint32_t)s.r.n * a.group;
         // Q fragments: row i * group + head of the group
         uint32_t qf[D / 16][4];
         int32_t pos[2], lo[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint32_t row = g + half * 8, i = min(row / a.group, (uint32_t)r.n - 1);
-            pos[half] = r.kv - r.n + (int32_t)i;
+            const uint32_t row = g + half * 8, i = min(row / a.group, (uint32_t)s.r.n - 1);
+            pos[half] = s.r.kv - s.r.n + (int32_t)i;
             lo[half] = window_begin(a, pos[half]);
-            const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + (int32_t)i) * a.q_token +
-                         (int64_t)(kvh * a.group + row % a.group) * a.q_head + t4 * 2;
+            const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.start + (int32_t)i) * a.q_token +
+                         (int64_t)(s.kvh * a.group + row % a.group) * a.q_head + t4 * 2;
+            const bool there = row < nrows;
+            if ((reinterpret_cast<uintptr_t>(q) & 3u) == 0) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                qf[k][half] = row < nrows ? load_pair<T>(q + k * 16) : 0u;
-                qf[k][half + 2] = row < nrows ? load_pair<T>(q + k * 16 + 8) : 0u;
+                for (int k = 0; k < D / 16; ++k) {
+                    qf[k][half] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
+                    qf[k][half + 2] = there ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+                }
+            } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(q);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    qf[k][half] = there ? (uint32_t)h[k * 16] | (uint32_t)h[k * 16 + 1] << 16 : 0u;
+                    qf[k][half + 2] = there ? (uint32_t)h[k * 16 + 8] | (uint32_t)h[k * 16 + 9] << 16 : 0u;
+                }
             }
         }
         float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -248,137 +362,96 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             for (int e = 0; e < 4; ++e)
                 o[n][e] = 0.0f;
 
-        // this warp's tiles: one of each block
-        const T* kb = reinterpret_cast<const T*>(a.c.k) + (int64_t)kvh * a.c.k_head;
-        const T* vb = reinterpret_cast<const T*>(a.c.v) + (int64_t)kvh * a.c.v_head;
-        auto tile_key = [&](uint32_t y) { return sp.key(y) + (int32_t)(warp * kDecTile); };
-        auto lookup = [&](uint32_t y) -> int32_t {
-            const int32_t j = tile_key(y);
-            return y < y1 && j < r.kv ? page_of(a, b, j) : -1;
-        };
-        // rows that no token sees arrive as zeros: whatever the cache holds
-        // there (a weight of zero times NaN is NaN) stays out of the product
-        auto fetch = [&](uint32_t y, uint32_t stage, int32_t page) {
-            const int32_t j0 = tile_key(y);
-            const uint32_t at = ring_addr + stage * kStage;
-            const int32_t in_page = j0 & ((1 << a.c.page_shift) - 1);
-            const T* kp = kb + (int64_t)max(page, 0) * a.c.k_page;
-            const T* vp = vb + (int64_t)max(page, 0) * a.c.v_page;
-#pragma unroll
-            for (uint32_t i = 0; i < kDecTile * kChunks / 32; ++i) {
-                const uint32_t row = i * (32 / kChunks) + lane / kChunks, chunk = lane % kChunks;
-                const int32_t j = j0 + (int32_t)row;
-                const bool take = page >= 0 && j < r.kv && (j >= sp.lo || j < sp.sink_end);
-                const uint32_t dst = at + row * (D * 2) + ((chunk ^ (row & 7u)) * 16u);
-                const int64_t off = take ? (int64_t)(in_page + (int32_t)row) : 0;
-                copy16(dst, take ? kp + off * a.c.k_row + chunk * 8 : kb, take);
-                copy16(dst + kDecTile * D * 2, take ? vp + off * a.c.v_row + chunk * 8 : vb, take);
-            }
-        };
-        int32_t page_ring[kStages];
-#pragma unroll
-        for (uint32_t s = 0; s < kStages; ++s)
-            page_ring[s] = lookup(y0 + s);
-#pragma unroll
-        for (uint32_t s = 0; s < kStages - 1; ++s) {
-            if (y0 + s < y1)
-                fetch(y0 + s, s, page_ring[s]);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        for (uint32_t yb = y0; yb < y1; yb += kStages) {
-#pragma unroll
-            for (uint32_t s = 0; s < kStages; ++s) {
-                const uint32_t y = yb + s;
-                if (y >= y1)
-                    break;
-                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-                __syncwarp();
-                const int32_t page = page_ring[s];
-                constexpr uint32_t kAhead = kStages - 1;
-                const uint32_t sn = (s + kAhead) % kStages;
-                if (y + kAhead < y1)
-                    fetch(y + kAhead, sn, page_ring[sn]);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                page_ring[s] = lookup(y + kStages);
+        uint32_t used = 0;  // the slot of the last tile
+#pragma unroll 1
+        for (uint32_t y = s.y0; y < s.y1; ++y) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            fetch();
+            const bool there = valid & 1u;
+            valid >>= 1;
+            --in_flight;
 
-                // S = Q K^T: two 8-key column tiles
-                const int32_t j0 = tile_key(y);
-                const uint32_t at = ring_addr + s * kStage;
-                float sc[2][4] = {};
-                {
-                    const uint32_t row = (lane & 7u) + ((lane >> 4) & 1u) * 8u;
+            // S = Q K^T: two 8-key column tiles
+            const int32_t j0 = tile_key(s, y);
+            const uint32_t at = ring_addr + slot * kStage;
+            used = slot;
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            float sc[2][4] = {};
+            {
+                const uint32_t row = (lane & 7u) + ((lane >> 4) & 1u) * 8u;
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        uint32_t kf[4];
-                        ldmatrix_x4(kf, at + row * (D * 2) + (((k * 2 + ((lane >> 3) & 1u)) ^ (row & 7u)) * 16u));
-                        mma_16816<T>(sc[0], qf[k], kf[0], kf[1]);
-                        mma_16816<T>(sc[1], qf[k], kf[2], kf[3]);
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t kf[4];
+                    ldmatrix_x4(kf, at + row * (D * 2) + (((k * 2 + ((lane >> 3) & 1u)) ^ (row & 7u)) * 16u));
+                    mma_16816<T>(sc[0], qf[k], kf[0], kf[1]);
+                    mma_16816<T>(sc[1], qf[k], kf[2], kf[3]);
+                }
+            }
+            const bool inside = there && j0 + (int32_t)kDecTile - 1 <= s.r.kv - s.r.n &&
+                                (a.window == 0 || j0 > s.r.kv - 1 - (int32_t)a.window);
+            if (!inside) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int32_t j = j0 + n * 8 + (int32_t)t4 * 2 + (e & 1);
+                        const bool seen = there && j <= pos[e >> 1] && (j >= lo[e >> 1] || j < (int32_t)a.sinks);
+                        sc[n][e] = seen ? sc[n][e] : -INFINITY;
                     }
-                }
-                const bool inside = page >= 0 && j0 + (int32_t)kDecTile - 1 <= r.kv - r.n &&
-                                    (a.window == 0 || j0 > r.kv - 1 - (int32_t)a.window);
-                if (!inside) {
+            }
+            // running maximum; O and l move with it
+            float mx[2];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int32_t j = j0 + n * 8 + (int32_t)t4 * 2 + (e & 1);
-                            const bool seen = page >= 0 && j <= pos[e >> 1] && (j >= lo[e >> 1] || j < (int32_t)a.sinks);
-                            sc[n][e] = seen ? sc[n][e] : -INFINITY;
-                        }
-                }
-                // running maximum; O and l move with it
-                float mx[2];
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    mx[h] = fmaxf(fmaxf(sc[0][2 * h], sc[0][2 * h + 1]), fmaxf(sc[1][2 * h], sc[1][2 * h + 1]));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                }
-                if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+                    const float mn = fmaxf(m[h], mx[h]);
+                    const float w = exp2_fast((m[h] - (mn == -INFINITY ? 0.0f : mn)) * a.scale_log2);
+                    m[h] = mn;
+                    l[h] *= w;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float mn = fmaxf(m[h], mx[h]);
-                        const float w = exp2_fast((m[h] - (mn == -INFINITY ? 0.0f : mn)) * a.scale_log2);
-                        m[h] = mn;
-                        l[h] *= w;
-#pragma unroll
-                        for (int n = 0; n < D / 8; ++n) {
-                            o[n][2 * h] *= w;
-                            o[n][2 * h + 1] *= w;
-                        }
-                    }
-                }
-                uint32_t pf[4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float base = m[h] == -INFINITY ? 0.0f : m[h];
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        p[e] = exp2_fast((sc[e >> 1][2 * h + (e & 1)] - base) * a.scale_log2);
-                    l[h] += (p[0] + p[1]) + (p[2] + p[3]);
-                    pf[h] = pack2<T>(p[0], p[1]);
-                    pf[h + 2] = pack2<T>(p[2], p[3]);
-                }
-                // O += P V
-                {
-                    const uint32_t row = (lane & 7u) + ((lane >> 3) & 1u) * 8u;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        uint32_t vf[4];
-                        ldmatrix_x4_trans(vf, at + kDecTile * D * 2 + row * (D * 2) +
-                                                  (((k * 2 + ((lane >> 4) & 1u)) ^ (row & 7u)) * 16u));
-                        mma_16816<T>(o[2 * k], pf, vf[0], vf[1]);
-                        mma_16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+                    for (int n = 0; n < D / 8; ++n) {
+                        o[n][2 * h] *= w;
+                        o[n][2 * h + 1] *= w;
                     }
                 }
             }
+            uint32_t pf[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float from = m[h] == -INFINITY ? 0.0f : m[h];
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    p[e] = exp2_fast((sc[e >> 1][2 * h + (e & 1)] - from) * a.scale_log2);
+                l[h] += (p[0] + p[1]) + (p[2] + p[3]);
+                pf[h] = pack2<T>(p[0], p[1]);
+                pf[h + 2] = pack2<T>(p[2], p[3]);
+            }
+            // O += P V
+            {
+                const uint32_t row = (lane & 7u) + ((lane >> 3) & 1u) * 8u;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    uint32_t vf[4];
+                    ldmatrix_x4_trans(vf, at + kDecTile * D * 2 + row * (D * 2) +
+                                              (((k * 2 + ((lane >> 4) & 1u)) ^ (row & 7u)) * 16u));
+                    mma_16816<T>(o[2 * k], pf, vf[0], vf[1]);
+                    mma_16816<T>(o[2 * k + 1], pf, vf[2], vf[3]);
+                }
+            }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+        // ---- the warps' parts: into the slots of the last tile (free until the
+        // next one is fetched), then one sum per value
         __syncwarp();
-
-        // ---- the warps' parts: into shared memory, then one sum per value
+        unsigned char* part_o = smem + used * kStage;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -387,147 +460,136 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 joint_m[warp][g + 8 * h] = m[h];
                 joint_l[warp][g + 8 * h] = l[h];
             }
-            float* po = reinterpret_cast<float*>(ring) + (g + 8 * h) * D + t4 * 2;
+            float* po = reinterpret_cast<float*>(part_o + warp * Shape::kWarpBytes) + (g + 8 * h) * D + t4 * 2;
             if (g + 8 * h < nrows)
 #pragma unroll
                 for (int n = 0; n < D / 8; ++n)
                     *reinterpret_cast<float2*>(po + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         }
-        if (tid == 0)
-            odd_rows = 0;
         __syncthreads();
 
-        // shares whose begin lies inside this row: c_lo .. c_hi
-        const uint64_t c_lo = row_begin * shares / total + 1;
-        uint64_t c_hi = row_end * shares / total;
-        while (c_hi >= c_lo && c_hi * total / shares >= row_end)
-            --c_hi;
-        uint64_t c_first = c_lo;
-        while (c_first <= c_hi && c_first * total / shares <= row_begin)
-            ++c_first;
-        const bool whole = sp.count <= kWholeBlocks || c_first > c_hi;
-        const uint32_t parts = whole ? 1u : (uint32_t)(c_hi - c_first + 2);
-        // the record of share c's part of a cut row: 1 if the row began in that share, else 0
-        float* record = a.partials + (2ull * blockIdx.x + (first_segment && y0 != 0 ? 0u : 1u)) * Shape::kRecord;
+        // shares that begin inside this row: c_first .. c_last
+        auto share_of = [&](uint32_t at) {
+            const uint32_t cut = extra * (even + 1);
+            return at < cut ? at / (even + 1) : extra + (at - cut) / even;
+        };
+        const uint32_t c_first = share_of(s.row_begin) + 1, c_last = share_of(s.row_begin + s.sp.count - 1);
+        const bool whole = s.sp.count <= kWholeBlocks || c_first > c_last;
+        const uint32_t parts = whole ? 1u : c_last - c_first + 2;
+        // the record of this share's part of a cut row: 1 if the row begins in this share, else 0
+        float* record = a.partials + (2ull * blockIdx.x + (s.y0 != 0 ? 0u : 1u)) * Shape::kRecord;
 
+#pragma unroll 1
         for (uint32_t idx = tid; idx < nrows * (D / 4); idx += kDecThreads) {
             const uint32_t row = idx / (D / 4), d = (idx % (D / 4)) * 4;
             float mm = joint_m[0][row];
 #pragma unroll
             for (uint32_t w = 1; w < kDecWarps; ++w)
                 mm = fmaxf(mm, joint_m[w][row]);
-            const float base = mm == -INFINITY ? 0.0f : mm;
-            float v[4] = {}, sum = 0.0f;
+            const float from = mm == -INFINITY ? 0.0f : mm;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float sum = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < kDecWarps; ++w) {
-                const float f = exp2_fast((joint_m[w][row] - base) * a.scale_log2);
-                const float4 p = *reinterpret_cast<const float4*>(smem + w * Shape::kWarpBytes + (row * D + d) * 4);
-                sum = __fmaf_rn(joint_l[w][row], f, sum);
-                v[0] = __fmaf_rn(p.x, f, v[0]);
-                v[1] = __fmaf_rn(p.y, f, v[1]);
-                v[2] = __fmaf_rn(p.z, f, v[2]);
-                v[3] = __fmaf_rn(p.w, f, v[3]);
+                const float e = exp2_fast((joint_m[w][row] - from) * a.scale_log2);
+                const float4 p = *reinterpret_cast<const float4*>(part_o + w * Shape::kWarpBytes + (row * D + d) * 4);
+                sum = __fmaf_rn(joint_l[w][row], e, sum);
+                v.x = __fmaf_rn(p.x, e, v.x);
+                v.y = __fmaf_rn(p.y, e, v.y);
+                v.z = __fmaf_rn(p.z, e, v.z);
+                v.w = __fmaf_rn(p.w, e, v.w);
             }
             if (whole) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = sum == 0.0f ? 0.0f : v[e] * inv;
-                    if (!finite32(v[e]))
-                        atomicOr(&odd_rows, 1u << row);
-                }
-                const uint32_t head = kvh * a.group + row % a.group, tok = (uint32_t)r.start + row / a.group;
-                store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
-                if (a.lse && d == 0)
-                    a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, logf(sum));
+                finish4<T>(a, (uint32_t)s.r.start + row / a.group, s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows, row);
             } else {
-                *reinterpret_cast<float4*>(record + 2 * kDecRows + row * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(record + 2 * kDecRows + row * D + d) = v;
                 if (d == 0) {
                     record[row] = mm;
                     record[kDecRows + row] = sum;
                 }
             }
         }
+        // ---- a cut row: the last of its shares to arrive joins all of them, in
+        // the order of the keys; more than kJoin parts first in groups of kJoin
+        // (one CTA reading hundreds of parts would take longer than the row)
         if (!whole) {
-            // ---- the last of the row's shares to arrive joins all of them
-            __threadfence();
-            __syncthreads();
-            int* counter = a.counters + (uint64_t)b * a.c.kv_heads + kvh;
-            if (tid == 0) {
-                const int before = atomicAdd(counter, 1);
-                last_arriver = before == (int)parts - 1;
-                if (last_arriver)
-                    *counter = 0;  // as the next call expects it
+            const uint32_t me = blockIdx.x - (c_first - 1), first_of_group = me / kJoin * kJoin;
+            const uint32_t groups = (parts + kJoin - 1) / kJoin;
+            // where the p-th part of this row, or the group that begins with it, has
+            // its record: a share ends one cut row (0) and begins another (1) at most
+            auto place = [&](uint32_t p) { return 2 * (c_first - 1 + p) + (p == 0 ? 1u : 0u); };
+#pragma unroll 1
+            for (uint32_t level = groups > 1 ? 0 : 1; level < 2; ++level) {
+                const bool grouped = level == 1 && groups > 1;
+                const uint32_t n = level == 0 ? min(kJoin, parts - first_of_group) : grouped ? groups : parts;
+                int* counter = level == 0 ? a.group_counters + place(first_of_group)
+                                          : a.row_counters + s.b * a.c.kv_heads + s.kvh;
                 __threadfence();
-            }
-            __syncthreads();
-            if (last_arriver) {
-                auto part = [&](uint32_t p) {  // in the order of the keys
-                    return a.partials + (p == 0 ? 2 * (c_first - 1) + 1 : 2 * (c_first - 1 + p)) * Shape::kRecord;
-                };
-                float* weight = reinterpret_cast<float*>(smem);  // [parts][nrows]
-                for (uint32_t row = warp; row < nrows; row += kDecWarps) {
-                    float mm = -INFINITY;
-                    for (uint32_t p = lane; p < parts; p += 32)
-                        mm = fmaxf(mm, __ldcg(part(p) + row));
-#pragma unroll
-                    for (int d = 16; d; d >>= 1)
-                        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-                    const float base = mm == -INFINITY ? 0.0f : mm;
-                    float sum = 0.0f;
-                    for (uint32_t p = lane; p < parts; p += 32) {
-                        const float f = exp2_fast((__ldcg(part(p) + row) - base) * a.scale_log2);
-                        weight[p * nrows + row] = f;
-                        sum = __fmaf_rn(__ldcg(part(p) + kDecRows + row), f, sum);
-                    }
-#pragma unroll
-                    for (int d = 16; d; d >>= 1)
-                        sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    if (lane == 0) {
-                        joint_l[0][row] = sum;
-                        joint_m[0][row] = mm;
-                    }
+                __syncthreads();
+                if (tid == 0) {
+                    last_arriver = atomicAdd(counter, 1) == (int)n - 1;
+                    if (last_arriver)
+                        *counter = 0;  // as the next call expects it
+                    __threadfence();
                 }
                 __syncthreads();
+                if (!last_arriver)
+                    break;
+                // record of the p-th of the n parts; the groups' lie behind the shares'
+                auto part = [&](uint32_t p) {
+                    return a.partials + (grouped ? 2ull * gridDim.x + place(p * kJoin)
+                                                 : (unsigned long long)place(level == 0 ? first_of_group + p : p)) * Shape::kRecord;
+                };
+                float* joined = a.partials + (2ull * gridDim.x + place(first_of_group)) * Shape::kRecord;
+#pragma unroll 1
                 for (uint32_t idx = tid; idx < nrows * (D / 4); idx += kDecThreads) {
                     const uint32_t row = idx / (D / 4), d = (idx % (D / 4)) * 4;
-                    float v[4] = {};
+                    float mm = -INFINITY, sum = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-                    for (uint32_t p = 0; p < parts; ++p) {
-                        const float f = weight[p * nrows + row];
+                    for (uint32_t p = 0; p < n; ++p)
+                        mm = fmaxf(mm, __ldcg(part(p) + row));
+                    const float from = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll 4
+                    for (uint32_t p = 0; p < n; ++p) {
+                        const float e = exp2_fast((__ldcg(part(p) + row) - from) * a.scale_log2);
                         const float4 q = __ldcg(reinterpret_cast<const float4*>(part(p) + 2 * kDecRows + row * D + d));
-                        v[0] = __fmaf_rn(q.x, f, v[0]);
-                        v[1] = __fmaf_rn(q.y, f, v[1]);
-                        v[2] = __fmaf_rn(q.z, f, v[2]);
-                        v[3] = __fmaf_rn(q.w, f, v[3]);
+                        sum = __fmaf_rn(__ldcg(part(p) + kDecRows + row), e, sum);
+                        v.x = __fmaf_rn(q.x, e, v.x);
+                        v.y = __fmaf_rn(q.y, e, v.y);
+                        v.z = __fmaf_rn(q.z, e, v.z);
+                        v.w = __fmaf_rn(q.w, e, v.w);
                     }
-                    const float sum = joint_l[0][row], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = sum == 0.0f ? 0.0f : v[e] * inv;
-                        if (!finite32(v[e]))
-                            atomicOr(&odd_rows, 1u << row);
+                    if (level == 1) {
+                        finish4<T>(a, (uint32_t)s.r.start + row / a.group, s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows,
+                                   row);
+                    } else {
+                        *reinterpret_cast<float4*>(joined + 2 * kDecRows + row * D + d) = v;
+                        if (d == 0) {
+                            joined[row] = mm;
+                            joined[kDecRows + row] = sum;
+                        }
                     }
-                    const uint32_t head = kvh * a.group + row % a.group, tok = (uint32_t)r.start + row / a.group;
-                    store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
-                    if (a.lse && d == 0)
-                        a.lse[(int64_t)tok * a.lse_token + head] =
-                            sum == 0.0f ? -INFINITY : __fmaf_rn(joint_m[0][row], a.scale, logf(sum));
                 }
             }
         }
         __syncthreads();
         // a row that came out infinite or NaN may owe it to a value that only
         // later tokens see: again, key by key (one token: every key counts)
-        const uint32_t odd = odd_rows;
-        if (odd != 0 && r.n > 1)
-            for (uint32_t row = warp; row < nrows; row += kDecWarps)
-                if (odd >> row & 1u)
-                    attention_row<D, T>(a, b, r, (int32_t)(row / a.group), kvh * a.group + row % a.group);
-        __syncthreads();
-        first_segment = false;
-        x = row_begin + y1;
+        if (const uint32_t odd = odd_rows) {
+            if (s.r.n > 1)
+#pragma unroll 1
+                for (uint32_t row = warp; row < nrows; row += kDecWarps)
+                    if (odd >> row & 1u)
+                        attention_row<D, T>(a, s.b, s.r, (int32_t)(row / a.group), s.kvh * a.group + row % a.group);
+            __syncthreads();
+            if (tid == 0)
+                odd_rows = 0;
+            __syncthreads();
+        }
+        x = s.row_begin + s.y1;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 }  // namespace paged

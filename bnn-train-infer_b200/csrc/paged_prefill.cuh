@@ -25,7 +25,7 @@
 
 #include "paged_common.cuh"
 #include "paged_decode.cuh"
-#include "w1a8_mma.cuh"
+#include "tcgen05.cuh"
 
 namespace bnn {
 namespace paged {
@@ -262,7 +262,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 if (round > 0)
-                    ok = mbar_wait(&empty[slot], (round - 1) & 1);
+                    ok = wait(&empty[slot], (round - 1) & 1);
                 if (!ok || starved)
                     break;
                 if (lane == 0) {
@@ -293,14 +293,14 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         // no copy may be in flight when the CTA exits
         const uint32_t issued = round * kStages + slot;
         for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-            if (!mbar_wait(&full[i % kStages], (i / kStages) & 1) && lane == 0)
+            if (!wait(&full[i % kStages], (i / kStages) & 1) && lane == 0)
                 atomicOr(a.status, kStatusTimeout);
     } else if (warp == kMmaWarp) {
         // ---- the products; tile by tile Q K^T of the next keys right after P V
         constexpr uint32_t kQkDesc = f16_idesc<T>(kPfKeys, false), kPvDesc = f16_idesc<T>(D, true);
         bool ok = true;
         auto need = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && mbar_wait(bar, parity);
+            ok = ok && wait(bar, parity);
             return ok;
         };
         auto slot_of = [&](uint32_t t, uint32_t which) { return (2 * t + which) % kStages; };
@@ -384,7 +384,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         }
         // the TMEM may go when every product issued has completed
         commit(drained);
-        if (!mbar_wait(drained, 0) && lane == 0)
+        if (!wait(drained, 0) && lane == 0)
             atomicOr(a.status, kStatusTimeout);
     } else {
         // ---- softmax: thread = row
@@ -394,7 +394,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         {
             unsigned char* q = q_sm + tile * kTileBytes;
             constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
-#pragma unroll 4
+#pragma unroll 2
             for (uint32_t i = 0; i < 32 / kAtOnce; ++i) {
                 const uint32_t in_warp = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
                 const uint32_t row = wrow + in_warp, tr = (warp % 4) * 32 + in_warp;
@@ -424,24 +424,34 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         bool ok = true;
         uint32_t t = 0;
         for (; t < count; ++t) {
-            if (!(ok = mbar_wait(&s_ready[tile], t & 1)))
+            if (!(ok = wait(&s_ready[tile], t & 1)))
                 break;
             tc_fence_after();
+            const int32_t key0 = tiles.key(t);
+            const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
+            if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
+                // at the edges of what the rows see: hidden scores to -inf, in place
+#pragma unroll 1
+                for (int32_t i = 0; i < (int32_t)kPfKeys; i += 32) {
+                    uint32_t s[32];
+                    tmem_ld32(t_s + i, s);
+                    tmem_wait();
+                    const int32_t hi = pos - key0 - i, low = lo - key0 - i, sink = (int32_t)a.sinks - key0 - i;
+                    const uint32_t part = bits >> (i / 16);
+#pragma unroll
+                    for (int32_t e = 0; e < 32; ++e) {
+                        const bool seen = e <= hi && (e >= low || e < sink) && (part >> (e / 16) & 1u);
+                        s[e] = seen ? s[e] : 0xff800000u;
+                    }
+                    tmem_st32(t_s + i, s);
+                }
+                tmem_wait_st();
+            }
             uint32_t s[kPfKeys];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
                 tmem_ld32(t_s + i * 32, s + i * 32);
             tmem_wait();
-            const int32_t key0 = tiles.key(t);
-            const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
-            if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
-                const int32_t hi = pos - key0, low = lo - key0, sink = (int32_t)a.sinks - key0;
-#pragma unroll
-                for (int32_t i = 0; i < (int32_t)kPfKeys; ++i) {
-                    const bool seen = i <= hi && (i >= low || i < sink) && (bits >> (i / 16) & 1u);
-                    s[i] = seen ? s[i] : 0xff800000u;
-                }
-            }
             float mx[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -458,7 +468,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 const float w = grow ? exp2_fast((m - mn) * c) : 1.0f;
                 if (t > 0) {
                     // the product of the last keys has completed (s_ready)
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t i = 0; i < D / 32; ++i) {
                         uint32_t o[32];
                         tmem_ld32(t_o + i * 32, o);
@@ -495,7 +505,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 mbar_arrive(&p_ready[tile]);
         }
         if (ok && count > 0)
-            ok = mbar_wait(&s_ready[tile], count & 1);
+            ok = wait(&s_ready[tile], count & 1);
         if (!ok && lane == 0)
             atomicOr(a.status, kStatusTimeout);
         if (ok) {
@@ -505,27 +515,37 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             const int64_t tok = r.start + (int64_t)(my_row / a.group);
             const int64_t at = tok * a.o_token + (int64_t)head * a.o_head;
             bool odd = false;
-#pragma unroll
+            unsigned char* to = a.out + at * 2;
+            const bool wide = a.out_type != kTypeF32 && (reinterpret_cast<uintptr_t>(to) & 15u) == 0;
+#pragma unroll 1
             for (uint32_t i = 0; i < D / 32; ++i) {
                 uint32_t o[32];
+                float x[32];
                 if (count > 0) {
                     tmem_ld32(t_o + i * 32, o);
                     tmem_wait();
                 }
-                if (my_row < rows)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        float x[4];
+                for (int e = 0; e < 32; ++e) {
+                    x[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+                    odd |= !finite32(x[e]);
+                }
+                if (my_row < rows && wide) {
 #pragma unroll
-                        for (int f = 0; f < 4; ++f) {
-                            x[f] = l == 0.0f ? 0.0f : __uint_as_float(o[e + f]) * inv;
-                            odd |= !finite32(x[f]);
-                        }
-                        store_out4<T>(a, at + i * 32 + e, x);
-                    }
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4*>(to + (i * 32 + e) * 2) =
+                            make_uint4(pack2<T>(x[e], x[e + 1]), pack2<T>(x[e + 2], x[e + 3]), pack2<T>(x[e + 4], x[e + 5]),
+                                       pack2<T>(x[e + 6], x[e + 7]));
+                } else if (my_row < rows) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        store_out4_any<T>(a, at + i * 32 + e, x[e], x[e + 1], x[e + 2], x[e + 3]);
+                }
+                __syncwarp();
             }
+            odd = odd && my_row < rows;
             if (a.lse && my_row < rows)
-                a.lse[tok * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, logf(l));
+                a.lse[tok * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, ln_fast(l));
             // a row that came out infinite or NaN may owe it to a value that
             // only later tokens see: again, key by key
             uint32_t again = __ballot_sync(0xffffffffu, odd);
