@@ -139,9 +139,9 @@ BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t strea
         return st;
     // no more CTAs than blocks there can be
     const uint64_t per_row = (((uint64_t)a.table_width << a.c.page_shift) + kDecBlock - 1) / kDecBlock + 1;
-    const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * per_row;
+    const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * (per_row + kRowCost);
     if (most > INT32_MAX)
-        return BNN_ENOTSUP;  // blocks are counted in 32 bits
+        return BNN_ENOTSUP;  // the shares' units are counted in 32 bits
     return launch(attention_split_kernel<D, T>, dim3((uint32_t)std::min<uint64_t>(split_grid(device), most)), kDecThreads, smem,
                   stream, a);
 }

@@ -33,6 +33,9 @@ constexpr uint32_t kDecBlock = kDecTile * kDecWarps;     // keys of a CTA's step
 constexpr uint32_t kDecPerSm = 2;                        // CTAs an SM holds
 constexpr uint32_t kWholeBlocks = 8;
 constexpr uint32_t kMinShare = 4;                        // blocks
+// A row's fixed work (its queries, the pipeline's start, the joint sum) in
+// units of the time a block takes: shares are equal in blocks plus rows.
+constexpr uint32_t kRowCost = 2;
 constexpr uint32_t kDecRows = 16;
 constexpr uint32_t kJoin = 16;                           // parts of a row that one CTA joins at a time
 
@@ -149,12 +152,14 @@ __device__ __noinline__ void finish4(const AttnArgs& a, uint32_t tok, uint32_t h
         a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, ln_fast(sum));
 }
 
-// One stretch of a share: blocks [y0, y1) of row (b, kvh), which spans blocks
-// [row_begin, row_begin + sp.count) of the call.
+// One stretch of a share: blocks [y0, y1) of row (b, kvh). The row's units begin
+// at row_begin, kRowCost of them before those of its blocks.
 struct Segment {
     Request r;
     Span sp;
     uint32_t b, kvh, row_begin, y0, y1;
+    __device__ __forceinline__ uint32_t row_end() const { return row_begin + kRowCost + sp.count; }
+    __device__ __forceinline__ uint32_t next() const { return row_begin + kRowCost + y1; }  // where its successor begins
 };
 
 template <int D, typename T>
@@ -163,7 +168,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     constexpr uint32_t kStages = Shape::kStages, kStage = Shape::kStageBytes;
     constexpr uint32_t kChunks = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) unsigned char smem[];
-    uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + Shape::kRingBytes);  // [batch + 1] blocks before a request
+    uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + Shape::kRingBytes);  // [batch + 1] units before a request
     __shared__ uint32_t warp_sum[kDecWarps];
     __shared__ float joint_m[kDecWarps][kDecRows], joint_l[kDecWarps][kDecRows];
     __shared__ uint32_t odd_rows;
@@ -174,7 +179,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     griddep_launch_dependents();
     griddep_wait();
 
-    // ---- blocks of every request, and this CTA's share of them
+    // ---- what every request costs, in units (kRowCost and one for each block of
+    // a row), and this CTA's share of it
     uint32_t total = 0;
 #pragma unroll 1
     for (uint32_t b0 = 0; b0 < a.batch; b0 += kDecThreads) {
@@ -184,7 +190,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             const Request r = load_request(a, b);
             if (r.n > (int32_t)a.max_q && blockIdx.x == 0)
                 atomicOr(a.status, kPagedRange);
-            x = few_rows(a, r) ? span_of(a, r).count * a.c.kv_heads : 0;
+            x = few_rows(a, r) ? (span_of(a, r).count + kRowCost) * a.c.kv_heads : 0;
         }
         uint32_t sum = x;
 #pragma unroll
@@ -216,9 +222,9 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     const uint32_t shares = min(gridDim.x, max((total + kMinShare - 1) / kMinShare, min(rows, total)));
     if (blockIdx.x >= shares)
         return;
-    const uint32_t even = total / shares, extra = total % shares;  // the first `extra` shares have one block more
+    const uint32_t even = total / shares, extra = total % shares;  // the first `extra` shares have one unit more
 
-    // the request that block x belongs to
+    // the request that unit x belongs to
     auto request_at = [&](uint32_t x) {
         uint32_t lo = 0, hi = a.batch;
 #pragma unroll 1
@@ -231,7 +237,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         }
         return lo;
     };
-    // first block of share c; inside a short row it moves to the row's start
+    // first unit of share c; inside a short row, or before a row's first block,
+    // it moves to the row's start
     auto raw_begin = [&](uint32_t c) { return c * even + min(c, extra); };
     uint32_t ends[2];
 #pragma unroll 1
@@ -239,8 +246,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         const uint32_t at = raw_begin(blockIdx.x + i);
         uint32_t begin = at;
         if (at < total) {
-            const uint32_t b = request_at(at), len = (prefix[b + 1] - prefix[b]) / a.c.kv_heads;
-            begin = len > kWholeBlocks ? at : at - (at - prefix[b]) % len;
+            const uint32_t b = request_at(at), len = (prefix[b + 1] - prefix[b]) / a.c.kv_heads, in = (at - prefix[b]) % len;
+            begin = len > kWholeBlocks + kRowCost && in > kRowCost ? at : at - in;
         }
         ends[0] = i == 0 ? begin : ends[0];
         ends[1] = begin;
@@ -253,11 +260,12 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         s.b = request_at(x);
         s.r = load_request(a, s.b);
         s.sp = span_of(a, s.r);
-        const uint32_t in = x - prefix[s.b];
-        s.kvh = in / s.sp.count;
-        s.y0 = in - s.kvh * s.sp.count;
-        s.row_begin = x - s.y0;
-        s.y1 = min(x_end - s.row_begin, s.sp.count);
+        const uint32_t in = x - prefix[s.b], len = s.sp.count + kRowCost;
+        s.kvh = in / len;
+        const uint32_t y = in - s.kvh * len;
+        s.row_begin = x - y;
+        s.y0 = y > kRowCost ? y - kRowCost : 0;
+        s.y1 = min(x_end - s.row_begin, len) - kRowCost;
         return s;
     };
 
@@ -265,8 +273,9 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     const uint32_t page_mask = (1u << a.c.page_shift) - 1u;
     auto tile_key = [&](const Segment& s, uint32_t y) { return s.sp.key(y) + (int32_t)(warp * kDecTile); };
 
-    // ---- what is fetched: the next tile is block fy of segment f; the lanes
-    // hold the pages of its 32 blocks from `base` on, and of the 32 after them
+    // ---- what is fetched: the next tile is block fy of segment f, whose units
+    // begin at fx; the lanes hold the pages of its 32 blocks from `base` on, and of
+    // the 32 after them
     Segment f = segment_at(x_begin);
     uint32_t fx = x_begin, fy = f.y0, base = fy, slot_f = 0;
     auto lookup = [&](uint32_t y) -> int32_t {
@@ -303,9 +312,9 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             valid |= (page >= 0 ? 1u : 0u) << in_flight;
             ++in_flight;
             slot_f = slot_f + 1 == kStages ? 0 : slot_f + 1;
-            ++fx;
             ++fy;
             if (fy == f.y1) {
+                fx = f.next();
                 if (fx < x_end) {
                     f = segment_at(fx);
                     fy = base = f.y0;
@@ -468,12 +477,12 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         }
         __syncthreads();
 
-        // shares that begin inside this row: c_first .. c_last
+        // shares that begin behind this row's first block: c_first .. c_last
         auto share_of = [&](uint32_t at) {
             const uint32_t cut = extra * (even + 1);
             return at < cut ? at / (even + 1) : extra + (at - cut) / even;
         };
-        const uint32_t c_first = share_of(s.row_begin) + 1, c_last = share_of(s.row_begin + s.sp.count - 1);
+        const uint32_t c_first = share_of(s.row_begin + kRowCost) + 1, c_last = share_of(s.row_end() - 1);
         const bool whole = s.sp.count <= kWholeBlocks || c_first > c_last;
         const uint32_t parts = whole ? 1u : c_last - c_first + 2;
         // the record of this share's part of a cut row: 1 if the row begins in this share, else 0
@@ -587,7 +596,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 odd_rows = 0;
             __syncthreads();
         }
-        x = s.row_begin + s.y1;
+        x = s.next();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
