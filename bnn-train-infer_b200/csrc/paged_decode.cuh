@@ -35,7 +35,7 @@ constexpr uint32_t kWholeBlocks = 8;
 constexpr uint32_t kMinShare = 4;                        // blocks
 // A row's fixed work (its queries, the pipeline's start, the joint sum) in
 // units of the time a block takes: shares are equal in blocks plus rows.
-constexpr uint32_t kRowCost = 2;
+constexpr uint32_t kRowCost = 3;
 constexpr uint32_t kDecRows = 16;
 constexpr uint32_t kJoin = 16;                           // parts of a row that one CTA joins at a time
 
@@ -49,7 +49,7 @@ struct DecodeShape {
     static_assert(kDecRows * D * 4 <= kWarpBytes, "a warp's O fits its ring");
 };
 
-inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * 4 + 16; }
+inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * (4 + sizeof(Request)); }
 
 // The 64-key blocks of a request that some of its new tokens see: the sinks'
 // blocks, then those from the first token's window on.
@@ -152,6 +152,14 @@ __device__ __noinline__ void finish4(const AttnArgs& a, uint32_t tok, uint32_t h
         a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, ln_fast(sum));
 }
 
+// Counts this CTA in: what its threads wrote before the barrier ahead of this
+// is visible to whoever counts last, and theirs to it.
+__device__ __forceinline__ int arrive(int* counter) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
+
 // One stretch of a share: blocks [y0, y1) of row (b, kvh). The row's units begin
 // at row_begin, kRowCost of them before those of its blocks.
 struct Segment {
@@ -162,6 +170,15 @@ struct Segment {
     __device__ __forceinline__ uint32_t next() const { return row_begin + kRowCost + y1; }  // where its successor begins
 };
 
+// A row of which this CTA's share has a part: its shares c_first - 1 .. and so on.
+struct Cut {
+    Segment s;
+    uint32_t c_first, parts, first_of_group, level, n;
+    // where the p-th part, or the group that begins with it, has its record: a
+    // share ends one cut row (0) and begins another (1) at most
+    __device__ __forceinline__ uint32_t place(uint32_t p) const { return 2 * (c_first - 1 + p) + (p == 0 ? 1u : 0u); }
+};
+
 template <int D, typename T>
 static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split_kernel(const __grid_constant__ AttnArgs a) {
     using Shape = DecodeShape<D>;
@@ -169,10 +186,11 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     constexpr uint32_t kChunks = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) unsigned char smem[];
     uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + Shape::kRingBytes);  // [batch + 1] units before a request
+    Request* requests = reinterpret_cast<Request*>(prefix + a.batch + 1);
     __shared__ uint32_t warp_sum[kDecWarps];
     __shared__ float joint_m[kDecWarps][kDecRows], joint_l[kDecWarps][kDecRows];
     __shared__ uint32_t odd_rows;
-    __shared__ int last_arriver;
+    __shared__ Cut cut[2];
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t g = lane >> 2, t4 = lane & 3;  // fragment row and column pair
@@ -188,6 +206,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         uint32_t x = 0;
         if (b < a.batch) {
             const Request r = load_request(a, b);
+            requests[b] = r;
             if (r.n > (int32_t)a.max_q && blockIdx.x == 0)
                 atomicOr(a.status, kPagedRange);
             x = few_rows(a, r) ? (span_of(a, r).count + kRowCost) * a.c.kv_heads : 0;
@@ -258,7 +277,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     auto segment_at = [&](uint32_t x) {
         Segment s;
         s.b = request_at(x);
-        s.r = load_request(a, s.b);
+        s.r = requests[s.b];
         s.sp = span_of(a, s.r);
         const uint32_t in = x - prefix[s.b], len = s.sp.count + kRowCost;
         s.kvh = in / len;
@@ -333,7 +352,29 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     for (uint32_t s = 0; s < kStages - 1; ++s)
         fetch();
 
-    uint32_t x = x_begin, slot = 0;
+    // a row that came out infinite or NaN may owe it to a value that only later
+    // tokens see: again, key by key (one token: every key counts)
+    auto redo = [&](const Segment& s, uint32_t first_bit) {
+        __syncthreads();
+        if (const uint32_t odd = odd_rows >> first_bit) {
+            if (s.r.n > 1)
+#pragma unroll 1
+                for (uint32_t row = warp; row < kDecRows; row += kDecWarps)
+                    if (odd >> row & 1u)
+                        attention_row<D, T>(a, s.b, s.r, (int32_t)(row / a.group), s.kvh * a.group + row % a.group);
+            __syncthreads();
+            if (tid == 0)
+                odd_rows &= (1u << first_bit) - 1u;
+            __syncthreads();
+        }
+    };
+    // the share whose stretch of units holds `at`
+    auto share_of = [&](uint32_t at) {
+        const uint32_t cut = extra * (even + 1);
+        return at < cut ? at / (even + 1) : extra + (at - cut) / even;
+    };
+
+    uint32_t x = x_begin, slot = 0, cuts = 0, cut_x[2] = {0, 0};
     while (x < x_end) {
         // ---- one segment
         const Segment s = segment_at(x);
@@ -388,13 +429,19 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             slot = slot + 1 == kStages ? 0 : slot + 1;
             float sc[2][4] = {};
             {
+                float odd[2][4] = {};  // the odd steps apart: half the chain of dependent products
                 const uint32_t row = (lane & 7u) + ((lane >> 4) & 1u) * 8u;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     uint32_t kf[4];
                     ldmatrix_x4(kf, at + row * (D * 2) + (((k * 2 + ((lane >> 3) & 1u)) ^ (row & 7u)) * 16u));
-                    mma_16816<T>(sc[0], qf[k], kf[0], kf[1]);
-                    mma_16816<T>(sc[1], qf[k], kf[2], kf[3]);
+                    mma_16816<T>(k & 1 ? odd[0] : sc[0], qf[k], kf[0], kf[1]);
+                    mma_16816<T>(k & 1 ? odd[1] : sc[1], qf[k], kf[2], kf[3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[0][e] += odd[0][e];
+                    sc[1][e] += odd[1][e];
                 }
             }
             const bool inside = there && j0 + (int32_t)kDecTile - 1 <= s.r.kv - s.r.n &&
@@ -478,13 +525,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         __syncthreads();
 
         // shares that begin behind this row's first block: c_first .. c_last
-        auto share_of = [&](uint32_t at) {
-            const uint32_t cut = extra * (even + 1);
-            return at < cut ? at / (even + 1) : extra + (at - cut) / even;
-        };
         const uint32_t c_first = share_of(s.row_begin + kRowCost) + 1, c_last = share_of(s.row_end() - 1);
         const bool whole = s.sp.count <= kWholeBlocks || c_first > c_last;
-        const uint32_t parts = whole ? 1u : c_last - c_first + 2;
         // the record of this share's part of a cut row: 1 if the row begins in this share, else 0
         float* record = a.partials + (2ull * blockIdx.x + (s.y0 != 0 ? 0u : 1u)) * Shape::kRecord;
 
@@ -518,87 +560,119 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 }
             }
         }
-        // ---- a cut row: the last of its shares to arrive joins all of them, in
-        // the order of the keys; more than kJoin parts first in groups of kJoin
-        // (one CTA reading hundreds of parts would take longer than the row)
         if (!whole) {
-            const uint32_t me = blockIdx.x - (c_first - 1), first_of_group = me / kJoin * kJoin;
-            const uint32_t groups = (parts + kJoin - 1) / kJoin;
-            // where the p-th part of this row, or the group that begins with it, has
-            // its record: a share ends one cut row (0) and begins another (1) at most
-            auto place = [&](uint32_t p) { return 2 * (c_first - 1 + p) + (p == 0 ? 1u : 0u); };
-#pragma unroll 1
-            for (uint32_t level = groups > 1 ? 0 : 1; level < 2; ++level) {
-                const bool grouped = level == 1 && groups > 1;
-                const uint32_t n = level == 0 ? min(kJoin, parts - first_of_group) : grouped ? groups : parts;
-                int* counter = level == 0 ? a.group_counters + place(first_of_group)
-                                          : a.row_counters + s.b * a.c.kv_heads + s.kvh;
-                __threadfence();
-                __syncthreads();
-                if (tid == 0) {
-                    last_arriver = atomicAdd(counter, 1) == (int)n - 1;
-                    if (last_arriver)
-                        *counter = 0;  // as the next call expects it
-                    __threadfence();
-                }
-                __syncthreads();
-                if (!last_arriver)
-                    break;
-                // record of the p-th of the n parts; the groups' lie behind the shares'
-                auto part = [&](uint32_t p) {
-                    return a.partials + (grouped ? 2ull * gridDim.x + place(p * kJoin)
-                                                 : (unsigned long long)place(level == 0 ? first_of_group + p : p)) * Shape::kRecord;
-                };
-                float* joined = a.partials + (2ull * gridDim.x + place(first_of_group)) * Shape::kRecord;
-#pragma unroll 1
-                for (uint32_t idx = tid; idx < nrows * (D / 4); idx += kDecThreads) {
-                    const uint32_t row = idx / (D / 4), d = (idx % (D / 4)) * 4;
-                    float mm = -INFINITY, sum = 0.0f;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (uint32_t p = 0; p < n; ++p)
-                        mm = fmaxf(mm, __ldcg(part(p) + row));
-                    const float from = mm == -INFINITY ? 0.0f : mm;
-#pragma unroll 4
-                    for (uint32_t p = 0; p < n; ++p) {
-                        const float e = exp2_fast((__ldcg(part(p) + row) - from) * a.scale_log2);
-                        const float4 q = __ldcg(reinterpret_cast<const float4*>(part(p) + 2 * kDecRows + row * D + d));
-                        sum = __fmaf_rn(__ldcg(part(p) + kDecRows + row), e, sum);
-                        v.x = __fmaf_rn(q.x, e, v.x);
-                        v.y = __fmaf_rn(q.y, e, v.y);
-                        v.z = __fmaf_rn(q.z, e, v.z);
-                        v.w = __fmaf_rn(q.w, e, v.w);
-                    }
-                    if (level == 1) {
-                        finish4<T>(a, (uint32_t)s.r.start + row / a.group, s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows,
-                                   row);
-                    } else {
-                        *reinterpret_cast<float4*>(joined + 2 * kDecRows + row * D + d) = v;
-                        if (d == 0) {
-                            joined[row] = mm;
-                            joined[kDecRows + row] = sum;
-                        }
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        // a row that came out infinite or NaN may owe it to a value that only
-        // later tokens see: again, key by key (one token: every key counts)
-        if (const uint32_t odd = odd_rows) {
-            if (s.r.n > 1)
-#pragma unroll 1
-                for (uint32_t row = warp; row < nrows; row += kDecWarps)
-                    if (odd >> row & 1u)
-                        attention_row<D, T>(a, s.b, s.r, (int32_t)(row / a.group), s.kvh * a.group + row % a.group);
+            // at most two: the row that an earlier share began, and the last one
+            cut_x[cuts == 0 ? 0 : 1] = x;
+            ++cuts;
             __syncthreads();
-            if (tid == 0)
-                odd_rows = 0;
-            __syncthreads();
+        } else {
+            redo(s, 0);
         }
         x = s.next();
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- cut rows: the last of a row's shares to arrive joins all of them, in
+    // the order of the keys; more than kJoin parts first in groups of kJoin (one
+    // CTA reading hundreds of parts would take longer than the row). A share
+    // arrives when all its work is done: the joint sums hold up no stream.
+    if (cuts == 0)
+        return;
+    if (tid < cuts) {
+        const Segment c = segment_at(cut_x[tid]);
+        Cut& k = cut[tid];
+        k.s = c;
+        k.c_first = share_of(c.row_begin + kRowCost) + 1;
+        k.parts = share_of(c.row_end() - 1) - k.c_first + 2;
+        k.first_of_group = (blockIdx.x - (k.c_first - 1)) / kJoin * kJoin;
+        k.level = k.parts > kJoin ? 0 : 1;
+    }
+#pragma unroll 1
+    for (uint32_t round = 0; round < 2; ++round) {
+        __syncthreads();  // the CTA's records are written
+        if (tid < cuts) {
+            Cut& k = cut[tid];
+            k.n = 0;
+            if (k.level == round || (round == 1 && k.level == 2)) {
+                const bool grouped = k.parts > kJoin;
+                const uint32_t n = round == 0 ? min(kJoin, k.parts - k.first_of_group)
+                                   : grouped ? (k.parts + kJoin - 1) / kJoin : k.parts;
+                int* counter = round == 0 ? a.group_counters + k.place(k.first_of_group)
+                                          : a.row_counters + k.s.b * a.c.kv_heads + k.s.kvh;
+                if (arrive(counter) == (int)n - 1) {
+                    *counter = 0;  // as the next call expects it
+                    k.n = n;
+                    k.level = round == 0 ? 2 : k.level;  // 2: this CTA joined the group and counts for it
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t i = 0; i < cuts; ++i) {
+            const Cut& k = cut[i];
+            const uint32_t n = k.n, nrows = (uint32_t)k.s.r.n * a.group;
+            if (n == 0)
+                continue;
+            // record of the p-th of the n parts; the groups' lie behind the shares'
+            const bool grouped = round == 1 && k.parts > kJoin;
+            const uint32_t p_begin = round == 0 ? k.first_of_group : 0, p_step = grouped ? kJoin : 1;
+            const float* records = a.partials + (grouped ? 2ull * gridDim.x * Shape::kRecord : 0ull);
+            float* joined = a.partials + (2ull * gridDim.x + k.place(k.first_of_group)) * Shape::kRecord;
+            // both rows at once where there are two and threads for them
+            const uint32_t quads = nrows * (D / 4);
+            const uint32_t turn = cuts == 2 && i == 1 && quads <= kDecThreads / 2 ? tid ^ (kDecThreads / 2) : tid;
+#pragma unroll 1
+            for (uint32_t idx = turn; idx < quads; idx += kDecThreads) {
+                const uint32_t row = idx / (D / 4), d = (idx % (D / 4)) * 4;
+                float mm = -INFINITY, sum = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                for (uint32_t p0 = 0; p0 < n; p0 += 8) {  // eight parts at once: their loads overlap
+                    float pm[8], pl[8];
+                    float4 q[8];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const bool there = p0 + e < n;
+                        const float* from = records + (uint64_t)k.place(p_begin + (there ? p0 + e : 0) * p_step) * Shape::kRecord;
+                        pm[e] = there ? __ldcg(from + row) : -INFINITY;
+                        pl[e] = there ? __ldcg(from + kDecRows + row) : 0.0f;
+                        q[e] = there ? __ldcg(reinterpret_cast<const float4*>(from + 2 * kDecRows + row * D + d))
+                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    }
+                    float to = mm;
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e)
+                        to = fmaxf(to, pm[e]);
+                    const float base = to == -INFINITY ? 0.0f : to, w = exp2_fast((mm - base) * a.scale_log2);
+                    mm = to;
+                    sum *= w;
+                    v = make_float4(v.x * w, v.y * w, v.z * w, v.w * w);
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const float f = exp2_fast((pm[e] - base) * a.scale_log2);
+                        sum = __fmaf_rn(pl[e], f, sum);
+                        v.x = __fmaf_rn(q[e].x, f, v.x);
+                        v.y = __fmaf_rn(q[e].y, f, v.y);
+                        v.z = __fmaf_rn(q[e].z, f, v.z);
+                        v.w = __fmaf_rn(q[e].w, f, v.w);
+                    }
+                }
+                if (round == 1) {
+                    finish4<T>(a, (uint32_t)k.s.r.start + row / a.group, k.s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows,
+                               row + 16 * i);
+                } else {
+                    *reinterpret_cast<float4*>(joined + 2 * kDecRows + row * D + d) = v;
+                    if (d == 0) {
+                        joined[row] = mm;
+                        joined[kDecRows + row] = sum;
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll 1
+    for (uint32_t i = 0; i < cuts; ++i)
+        redo(cut[i].s, 16 * i);
 }
 
 }  // namespace paged
