@@ -10,6 +10,7 @@
 #pragma once
 
 #include "paged_common.cuh"
+#include "tcgen05.cuh"
 
 namespace bnn {
 namespace paged {
@@ -46,110 +47,147 @@ __device__ __forceinline__ float4 load4(const S* p, bool aligned) {
     }
 }
 
-// One warp: kHeads consecutive heads (per lane group) of one token's
-// q heads, k heads, v heads in this order.
+// One warp: up to kHeads (times the heads side by side in a warp) consecutive
+// heads of one kind (q, k or v) of one token; blockIdx.y counts these parts,
+// the q heads' first. Two values at a time (f32x2) where both are treated alike.
 template <int D, typename S, typename T, bool kInterleaved, int kHeads>
-static __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendArgs a) {
-    constexpr int kLanes = D / 4;           // lanes of a head
-    constexpr int kPer = 32 / kLanes;       // heads side by side in a warp
+static __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+    constexpr uint32_t kLanes = D / 4;           // lanes of a head
+    constexpr uint32_t kPer = 32 / kLanes;       // heads side by side in a warp
+    constexpr uint32_t kPart = kHeads * kPer;
     const uint32_t lane = threadIdx.x & 31, in = lane % kLanes;
-    const uint32_t all = a.heads + 2 * a.c.kv_heads;
-    const uint32_t parts = (all + kHeads * kPer - 1) / (kHeads * kPer);
-    const uint32_t warp = blockIdx.x * (kAppendThreads / 32) + threadIdx.x / 32;
-    const uint32_t t = warp / parts;
+    const uint32_t t = blockIdx.x * (kAppendThreads / 32) + threadIdx.x / 32;
     griddep_launch_dependents();
     if (t >= a.tokens)
         return;
-    const uint32_t h0 = (warp % parts) * (kHeads * kPer) + lane / kLanes;
+    const uint32_t q_parts = (a.heads + kPart - 1) / kPart, kv_parts = (a.c.kv_heads + kPart - 1) / kPart;
+    const int which = blockIdx.y < q_parts ? 0 : blockIdx.y < q_parts + kv_parts ? 1 : 2;
+    const uint32_t part = blockIdx.y - (which == 0 ? 0 : which == 1 ? q_parts : q_parts + kv_parts);
+    const uint32_t heads = which == 0 ? a.heads : a.c.kv_heads;
+    const uint32_t h0 = part * kPart + lane / kLanes;
+    const uint32_t e0 = in * 4;  // this lane's first dimension
     griddep_wait();
+
+    float4 x[kHeads];
+    {
+        const int64_t step = (int64_t)kPer * a.head[which];
+        const S* p = reinterpret_cast<const S*>(a.src[which]) + (int64_t)t * a.token[which] + (int64_t)h0 * a.head[which] + e0;
+        const bool aligned = ((reinterpret_cast<uintptr_t>(p) | (uint64_t)step * sizeof(S)) & (4 * sizeof(S) - 1)) == 0;
+        if (aligned) {
+#pragma unroll
+            for (int u = 0; u < kHeads; ++u)
+                x[u] = h0 + u * kPer < heads ? load4<S>(p + u * step, true) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kHeads; ++u)
+                x[u] = h0 + u * kPer < heads ? load4<S>(p + u * step, false) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
     const int32_t pos = a.positions[t], slot = a.slots[t];
     const bool pos_ok = a.rotary == 0 || (uint32_t)pos < a.table_rows;
     const int64_t room = (int64_t)a.c.pages << a.c.page_shift;
-    const bool stored = pos_ok && slot >= 0 && slot < room;
-    if (lane == 0 && (!pos_ok || slot >= room))
+    if (blockIdx.y == 0 && lane == 0 && (!pos_ok || slot >= room))
         atomicOr(a.status, kPagedRange);
-    const uint32_t e0 = in * 4;  // this lane's first dimension
 
-    float4 x[kHeads];
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-        const uint32_t h = h0 + u * kPer;
-        if (h < all) {
-            const int which = h < a.heads ? 0 : h < a.heads + a.c.kv_heads ? 1 : 2;
-            const uint32_t hh = which == 0 ? h : which == 1 ? h - a.heads : h - a.heads - a.c.kv_heads;
-            const S* p = reinterpret_cast<const S*>(a.src[which]) + (int64_t)t * a.token[which] +
-                         (int64_t)hh * a.head[which] + e0;
-            x[u] = load4<S>(p, (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(S) - 1)) == 0);
-        } else {
-            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-    }
-    // this lane's factors of the rotation
-    const uint32_t half = a.rotary / 2;
-    const bool turned = e0 < a.rotary && pos_ok;
-    float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    uint32_t partner = lane;
-    if (turned) {
-        const int64_t at = (int64_t)pos * half;
-        if (kInterleaved) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                c[2 * e] = c[2 * e + 1] = a.cos[at + e0 / 2 + e];
-                s[2 * e + 1] = a.sin[at + e0 / 2 + e];
-                s[2 * e] = -s[2 * e + 1];
+    if (which < 2) {
+        // this lane's factors of the rotation
+        const uint32_t half = a.rotary / 2;
+        const bool turned = e0 < a.rotary && pos_ok;
+        uint64_t c[2] = {f2_pack(1.0f, 1.0f), f2_pack(1.0f, 1.0f)}, s[2] = {0, 0};
+        uint32_t partner = lane;
+        if (turned) {
+            const int64_t at = (int64_t)pos * half;
+            if (kInterleaved) {
+                const float2 cc = *reinterpret_cast<const float2*>(a.cos + at + e0 / 2);
+                const float2 ss = *reinterpret_cast<const float2*>(a.sin + at + e0 / 2);
+                c[0] = f2_pack(cc.x, cc.x);
+                c[1] = f2_pack(cc.y, cc.y);
+                s[0] = f2_pack(-ss.x, ss.x);
+                s[1] = f2_pack(-ss.y, ss.y);
+            } else {
+                const bool first = e0 < half;
+                const uint32_t i = first ? e0 : e0 - half;
+                const float4 cc = *reinterpret_cast<const float4*>(a.cos + at + i);
+                const float4 ss = *reinterpret_cast<const float4*>(a.sin + at + i);
+                const float sign = first ? -1.0f : 1.0f;
+                c[0] = f2_pack(cc.x, cc.y);
+                c[1] = f2_pack(cc.z, cc.w);
+                s[0] = f2_pack(sign * ss.x, sign * ss.y);
+                s[1] = f2_pack(sign * ss.z, sign * ss.w);
+                partner = first ? lane + half / 4 : lane - half / 4;
             }
-        } else {
-            const bool first = e0 < half;
-            const uint32_t i = first ? e0 : e0 - half;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                c[e] = a.cos[at + i + e];
-                s[e] = first ? -a.sin[at + i + e] : a.sin[at + i + e];
-            }
-            partner = first ? lane + half / 4 : lane - half / 4;
         }
-    }
-#pragma unroll
-    for (int u = 0; u < kHeads; ++u) {
-        const uint32_t h = h0 + u * kPer;
-        const int which = h < a.heads ? 0 : h < a.heads + a.c.kv_heads ? 1 : 2;
-        float4 y = x[u];
-        const float* gain = which < 2 ? a.gain[which] : nullptr;
-        float sq = __fmaf_rn(y.x, y.x, __fmaf_rn(y.y, y.y, __fmaf_rn(y.z, y.z, y.w * y.w)));
-#pragma unroll
-        for (int d = 1; d < kLanes; d <<= 1)
-            sq += __shfl_xor_sync(0xffffffffu, sq, d);
+        // 1 / rms of each head. The heads' sums are reduced together: each exchange
+        // halves the values a lane carries until one is left, so kHeads butterflies
+        // cost little more than one, and one root is taken per lane
+        const float* gain = a.gain[which];
         if (gain) {
-            const float4 g = *reinterpret_cast<const float4*>(gain + e0);
-            const float inv = 1.0f / sqrtf(__fmaf_rn(sq, 1.0f / D, a.eps));
-            y = make_float4(y.x * inv * g.x, y.y * inv * g.y, y.z * inv * g.z, y.w * inv * g.w);
+            float sq[kHeads];
+#pragma unroll
+            for (int u = 0; u < kHeads; ++u) {
+                const uint64_t lo = f2_pack(x[u].x, x[u].y), hi = f2_pack(x[u].z, x[u].w);
+                const uint64_t q = f2_fma(lo, lo, f2_mul(hi, hi));
+                sq[u] = f2_lo(q) + f2_hi(q);
+            }
+            uint32_t d = kLanes / 2;
+#pragma unroll
+            for (int n = kHeads; n > 1; n >>= 1, d >>= 1) {
+                const bool upper = in & d;
+#pragma unroll
+                for (int u = 0; u < n / 2; ++u) {
+                    const float keep = upper ? sq[u + n / 2] : sq[u], give = upper ? sq[u] : sq[u + n / 2];
+                    sq[u] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+                }
+            }
+#pragma unroll
+            for (; d; d >>= 1)
+                sq[0] += __shfl_xor_sync(0xffffffffu, sq[0], d);
+            const float r = rsqrtf(__fmaf_rn(sq[0], 1.0f / D, a.eps));  // off by 2 ulp: far below the 16-bit rounding
+            const float4 g4 = *reinterpret_cast<const float4*>(gain + e0);
+            const uint64_t g[2] = {f2_pack(g4.x, g4.y), f2_pack(g4.z, g4.w)};
+#pragma unroll
+            for (int u = 0; u < kHeads; ++u) {
+                const float inv = __shfl_sync(0xffffffffu, r, (lane & ~(kLanes - 1u)) + u * (kLanes / kHeads));
+                const uint64_t i2 = f2_pack(inv, inv);
+                const uint64_t lo = f2_mul(f2_mul(f2_pack(x[u].x, x[u].y), i2), g[0]);
+                const uint64_t hi = f2_mul(f2_mul(f2_pack(x[u].z, x[u].w), i2), g[1]);
+                x[u] = make_float4(f2_lo(lo), f2_hi(lo), f2_lo(hi), f2_hi(hi));
+            }
         }
-        float4 o = make_float4(y.y, y.x, y.w, y.z);  // the pairs' other values
-        if (!kInterleaved) {
-            o.x = __shfl_sync(0xffffffffu, y.x, partner);
-            o.y = __shfl_sync(0xffffffffu, y.y, partner);
-            o.z = __shfl_sync(0xffffffffu, y.z, partner);
-            o.w = __shfl_sync(0xffffffffu, y.w, partner);
-        }
-        if (which < 2 && turned)
-            y = make_float4(__fmaf_rn(y.x, c[0], o.x * s[0]), __fmaf_rn(y.y, c[1], o.y * s[1]),
-                            __fmaf_rn(y.z, c[2], o.z * s[2]), __fmaf_rn(y.w, c[3], o.w * s[3]));
-        if (h >= all)
-            continue;
-        uint2 w = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
-        if (which == 0) {
-            if (!pos_ok)
-                w = make_uint2(0u, 0u);
-            T* p = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.o_token + (int64_t)h * a.o_head + e0;
-            *reinterpret_cast<uint2*>(p) = w;
-        } else if (stored) {
-            const uint32_t hh = which == 1 ? h - a.heads : h - a.heads - a.c.kv_heads;
-            const int64_t page = slot >> a.c.page_shift, row = slot & ((1 << a.c.page_shift) - 1);
-            const int64_t at = which == 1 ? page * a.c.k_page + (int64_t)hh * a.c.k_head + row * a.c.k_row
-                                          : page * a.c.v_page + (int64_t)hh * a.c.v_head + row * a.c.v_row;
-            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(which == 1 ? a.c.k : a.c.v) + at + e0) = w;
+        if (a.rotary != 0) {
+#pragma unroll
+            for (int u = 0; u < kHeads; ++u) {
+                float4 o = make_float4(x[u].y, x[u].x, x[u].w, x[u].z);  // the pairs' other values
+                if (!kInterleaved)
+                    o = make_float4(__shfl_sync(0xffffffffu, x[u].x, partner), __shfl_sync(0xffffffffu, x[u].y, partner),
+                                    __shfl_sync(0xffffffffu, x[u].z, partner), __shfl_sync(0xffffffffu, x[u].w, partner));
+                if (turned) {
+                    const uint64_t lo = f2_fma(f2_pack(x[u].x, x[u].y), c[0], f2_mul(f2_pack(o.x, o.y), s[0]));
+                    const uint64_t hi = f2_fma(f2_pack(x[u].z, x[u].w), c[1], f2_mul(f2_pack(o.z, o.w), s[1]));
+                    x[u] = make_float4(f2_lo(lo), f2_hi(lo), f2_lo(hi), f2_hi(hi));
+                }
+            }
         }
     }
+    T* to;
+    int64_t step;
+    if (which == 0) {
+        step = (int64_t)kPer * a.o_head;
+        to = reinterpret_cast<T*>(a.q_out) + (int64_t)t * a.o_token + (int64_t)h0 * a.o_head + e0;
+    } else {
+        if (!pos_ok || slot < 0 || slot >= room)
+            return;
+        const int64_t page = slot >> a.c.page_shift, row = slot & ((1 << a.c.page_shift) - 1);
+        const int64_t head = which == 1 ? a.c.k_head : a.c.v_head;
+        step = (int64_t)kPer * head;
+        to = reinterpret_cast<T*>(which == 1 ? a.c.k : a.c.v) + page * (which == 1 ? a.c.k_page : a.c.v_page) +
+             row * (which == 1 ? a.c.k_row : a.c.v_row) + (int64_t)h0 * head + e0;
+    }
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u)
+        if (h0 + u * kPer < heads)
+            *reinterpret_cast<uint2*>(to + u * step) =
+                pos_ok ? make_uint2(pack2<T>(x[u].x, x[u].y), pack2<T>(x[u].z, x[u].w)) : make_uint2(0u, 0u);
 }
 
 }  // namespace paged

@@ -59,7 +59,7 @@ typedef struct {
  * norm where the gain is NULL), then dimensions below rotary_dim rotated by
  * row positions[t] of the cos/sin tables [table_rows][rotary_dim / 2]:
  * (a, b) -> (a cos - b sin, b cos + a sin) over pairs (i, i + rotary_dim / 2),
- * or (2i, 2i + 1) with interleaved != 0. All in FP32, rounded once to the
+ * or (2i, 2i + 1) with interleaved != 0 (gains and tables on 16-byte boundaries). All in FP32, rounded once to the
  * cache's type. q goes to q_out (same type as the cache), k and v to slot
  * slots[t]; a negative slot stores neither. rotary_dim: 0, or a multiple of 8
  * up to head_dim. A position outside the table leaves the token's q_out rows
