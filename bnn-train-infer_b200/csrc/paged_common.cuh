@@ -141,11 +141,18 @@ __device__ __forceinline__ float ln_fast(float x) {
     return y * 0.693147182f;
 }
 
-// mbar_wait (bnn_sync.cuh) with the waiting itself out of line: these kernels
-// wait at many places, and a call of few tiles runs each once.
+// mbar_wait (bnn_sync.cuh) behind a number of plain polls: these kernels hand
+// over every microsecond, and the polls that sleep and read the timer see a
+// finished phase later. The slow part is out of line: there are many waits, and
+// a call of few tiles runs each once.
+constexpr uint32_t kQuickPolls = 64;
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity); }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-    return mbar_try_wait(bar, parity) || wait_slow(bar, parity);
+#pragma unroll 1
+    for (uint32_t i = 0; i < kQuickPolls; ++i)
+        if (mbar_try_wait(bar, parity))
+            return true;
+    return wait_slow(bar, parity);
 }
 
 // The whole of one output row by one warp, straight from the definition: a

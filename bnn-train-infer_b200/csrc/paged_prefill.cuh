@@ -31,6 +31,7 @@ namespace bnn {
 namespace paged {
 
 constexpr uint32_t kPfKeys = 128;   // keys of a tile
+constexpr uint32_t kPfHalf = 64;    // keys whose weights are handed over at once
 constexpr uint32_t kPfRows = 128;   // rows of a tile
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
 
@@ -41,7 +42,7 @@ struct PrefillShape {
     static constexpr uint32_t kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 4 : 8);
     static constexpr uint32_t kTmemUsed = kTiles * (kPfKeys + D);
     static constexpr uint32_t kTmemCols = kTmemUsed <= 256 ? 256 : 512;
-    static constexpr uint32_t kBars = 2 * kStages + 3 * kTiles + 1;
+    static constexpr uint32_t kBars = 2 * kStages + 4 * kTiles + 1;
     static constexpr size_t kSmem = 1024 + (size_t)(kTiles + kStages) * kTileBytes + kBars * 8 + 16 * 4 + 64;
 };
 
@@ -85,6 +86,22 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
         : "memory");
 }
 
+// True in one thread of the (whole) warp. A tcgen05.mma takes its operands from
+// uniform registers: behind this test the compiler knows that one thread runs
+// and keeps them there; behind lane == 0 it does not, and each product cost
+// some 130 clocks to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// Eight adjacent 16-bit values at any 2-byte alignment.
+template <typename T>
+__device__ __noinline__ uint4 load_row16(const T* p) {
+    return make_uint4(load_pair<T>(p), load_pair<T>(p + 2), load_pair<T>(p + 4), load_pair<T>(p + 6));
+}
+
 // 32 words to consecutive TMEM columns of this warp's lanes; complete after tmem_wait_st().
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
     asm volatile(
@@ -112,6 +129,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+
+// The lowest n bits (none below 1, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // Key tiles that rows of tokens at positions p0 .. p1 see.
 struct KeyTiles {
@@ -151,9 +171,9 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kTileBytes);
     uint64_t* empty = full + kStages;
     uint64_t* q_ready = empty + kStages;     // [kTiles] Q in shared memory
-    uint64_t* s_ready = q_ready + kTiles;    // [kTiles] S in TMEM and the product before it done; at the end O complete
-    uint64_t* p_ready = s_ready + kTiles;    // [kTiles] P in TMEM, O scaled
-    uint64_t* drained = p_ready + kTiles;
+    uint64_t* s_ready = q_ready + kTiles;    // [kTiles] S in TMEM and the last keys' P V done
+    uint64_t* p_ready = s_ready + kTiles;    // [kTiles][2] half of P in TMEM, O scaled
+    uint64_t* drained = p_ready + 2 * kTiles;
     uint32_t* mapped = reinterpret_cast<uint32_t*>(drained + 1);  // [16] bit u: 16-key part u of tile t (mod 16) is in memory
     uint32_t* tmem_slot = mapped + 16;
     __shared__ uint32_t warp_sum[32];
@@ -169,7 +189,8 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         for (int t = 0; t < kTiles; ++t) {
             mbar_init(&q_ready[t], 4);
             mbar_init(&s_ready[t], 1);
-            mbar_init(&p_ready[t], 4);
+            mbar_init(&p_ready[2 * t], 4);
+            mbar_init(&p_ready[2 * t + 1], 4);
         }
         mbar_init(drained, 1);
         fence_barrier_init();
@@ -231,7 +252,6 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     const KeyTiles tiles = key_tiles(a, base_pos + (int32_t)(row0 / a.group),
                                      base_pos + (int32_t)(min(row0 + kItemRows, rows) - 1) / (int32_t)a.group);
     const uint32_t count = tiles.count;
-
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                      "r"(Shape::kTmemCols));
@@ -296,94 +316,68 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             if (!wait(&full[i % kStages], (i / kStages) & 1) && lane == 0)
                 atomicOr(a.status, kStatusTimeout);
     } else if (warp == kMmaWarp) {
-        // ---- the products; tile by tile Q K^T of the next keys right after P V
-        constexpr uint32_t kQkDesc = f16_idesc<T>(kPfKeys, false), kPvDesc = f16_idesc<T>(D, true);
-        bool ok = true;
-        auto need = [&](uint64_t* bar, uint32_t parity) {
-            ok = ok && wait(bar, parity);
-            return ok;
-        };
-        auto slot_of = [&](uint32_t t, uint32_t which) { return (2 * t + which) % kStages; };
-        auto parity_of = [&](uint32_t t, uint32_t which) { return ((2 * t + which) / kStages) & 1; };
-        auto qk = [&](uint32_t tile, uint32_t t) {
-            if (lane == 0) {
-                const uint32_t qa = smem_addr(q_sm) + tile * kTileBytes;
-                const uint32_t ka = smem_addr(ring) + slot_of(t, 0) * kTileBytes;
+        // ---- the products, all by one thread; Q K^T of the next keys right after P V
+        if (elect_one()) {
+            constexpr uint32_t kQkDesc = f16_idesc<T>(kPfKeys, false), kPvDesc = f16_idesc<T>(D, true);
+            const uint64_t q_desc = mma_smem_desc(smem_addr(q_sm)), k_desc = mma_smem_desc(smem_addr(ring));
+            const uint64_t v_desc = mn_smem_desc(smem_addr(ring));
+            bool ok = true;
+            auto need = [&](uint64_t* bar, uint32_t parity) {
+                ok = ok && wait(bar, parity);
+                return ok;
+            };
+            auto slot_of = [&](uint32_t t, uint32_t which) { return (2 * t + which) % kStages; };
+            auto parity_of = [&](uint32_t t, uint32_t which) { return ((2 * t + which) / kStages) & 1; };
+            auto qk = [&](uint32_t tile, uint32_t t) {
+                const uint64_t qa = q_desc + (tile * kTileBytes >> 4), ka = k_desc + (slot_of(t, 0) * kTileBytes >> 4);
+                const uint32_t to = tmem + tile * kPfKeys;
 #pragma unroll
                 for (uint32_t k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k / 4) * kHalfBytes + (k % 4) * 32;
-                    mma_f16_ss(tmem + tile * kPfKeys, mma_smem_desc(qa + off), mma_smem_desc(ka + off), kQkDesc, k != 0);
+                    const uint32_t off = ((k / 4) * kHalfBytes + (k % 4) * 32) >> 4;
+                    mma_f16_ss(to, qa + off, ka + off, kQkDesc, k != 0);
                 }
-            }
-        };
-        auto pv = [&](uint32_t tile, uint32_t t) {
-            if (lane == 0) {
-                const uint32_t va = smem_addr(ring) + slot_of(t, 1) * kTileBytes;
-#pragma unroll
-                for (uint32_t k = 0; k < kPfKeys / 16; ++k)
-                    mma_f16_ts(tmem_o + tile * D, tmem + tile * kPfKeys + k * 8, mn_smem_desc(va + k * 16 * 128), kPvDesc,
-                               t != 0 || k != 0);
-            }
-        };
-        auto commit = [&](uint64_t* bar) {
-            if (lane == 0)
-                mma_commit(bar);
-        };
-        if (count > 0 && need(&full[slot_of(0, 0)], 0)) {
-#pragma unroll
-            for (uint32_t tile = 0; tile < kTiles; ++tile) {
-                if (!need(&q_ready[tile], 0))
-                    break;
-                tc_fence_after();
-                qk(tile, 0);
-                commit(&s_ready[tile]);
-            }
-            commit(&empty[slot_of(0, 0)]);
-            for (uint32_t t = 0; ok && t < count; ++t) {
-                if (!need(&full[slot_of(t, 1)], parity_of(t, 1)))
-                    break;
-                // V rows that no row of this CTA sees: zeros
-                const int32_t key0 = tiles.key(t);
-                const uint32_t bits = mapped[t % 16];
-                if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > tiles.last || key0 < tiles.lo) {
-                    unsigned char* v = ring + slot_of(t, 1) * kTileBytes;
-                    for (uint32_t row = lane / 8; row < kPfKeys; row += 4) {
-                        const int32_t j = key0 + (int32_t)row;
-                        const bool used = (bits >> (row / 16) & 1u) && j <= tiles.last && (j >= tiles.lo || j < tiles.sink_end);
-                        if (!used)
-#pragma unroll
-                            for (uint32_t h = 0; h < kHalves; ++h)
-                                *reinterpret_cast<uint4*>(v + h * kHalfBytes + row * 128 + (lane % 8) * 16) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async();
-                    __syncwarp();
-                }
-                if (t + 1 < count && !need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0)))
-                    break;
-#pragma unroll
-                for (uint32_t tile = 0; tile < kTiles; ++tile) {
-                    if (!need(&p_ready[tile], t & 1))
-                        break;
+            };
+            if (count > 0 && need(&full[slot_of(0, 0)], 0)) {
+#pragma unroll 1
+                for (uint32_t tile = 0; tile < kTiles && need(&q_ready[tile], 0); ++tile) {
                     tc_fence_after();
-                    pv(tile, t);
-                    if (tile == kTiles - 1)
-                        commit(&empty[slot_of(t, 1)]);
-                    if (t + 1 < count) {
-                        qk(tile, t + 1);
-                        if (tile == kTiles - 1)
-                            commit(&empty[slot_of(t + 1, 0)]);
+                    qk(tile, 0);
+                    mma_commit(&s_ready[tile]);
+                }
+                mma_commit(&empty[slot_of(0, 0)]);
+#pragma unroll 1
+                for (uint32_t t = 0; ok && t < count; ++t) {
+                    const bool more = t + 1 < count;
+                    if (!need(&full[slot_of(t, 1)], parity_of(t, 1)))
+                        break;
+                    const uint64_t va = v_desc + (slot_of(t, 1) * kTileBytes >> 4);
+#pragma unroll 1
+                    for (uint32_t tile = 0; ok && tile < kTiles; ++tile) {
+#pragma unroll 1
+                        for (uint32_t h = 0; h < 2 && need(&p_ready[2 * tile + h], t & 1); ++h) {
+                            tc_fence_after();
+#pragma unroll
+                            for (uint32_t k = 0; k < kPfHalf / 16; ++k)
+                                mma_f16_ts(tmem_o + tile * D, tmem + tile * kPfKeys + h * (kPfHalf / 2) + k * 8,
+                                           va + ((h * kPfHalf + k * 16) * 128 >> 4), kPvDesc, t != 0 || h != 0 || k != 0);
+                        }
+                        if (!ok || (more && tile == 0 && !need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0))))
+                            break;
+                        if (more)
+                            qk(tile, t + 1);
+                        mma_commit(&s_ready[tile]);
                     }
-                    commit(&s_ready[tile]);
+                    mma_commit(&empty[slot_of(t, 1)]);
+                    if (more)
+                        mma_commit(&empty[slot_of(t + 1, 0)]);
                 }
             }
-            if (!ok && lane == 0)
+            if (!ok)
                 atomicOr(a.status, kStatusTimeout);
-        } else if (!ok && lane == 0) {
-            atomicOr(a.status, kStatusTimeout);
+            // the TMEM may go when every product issued has completed
+            mma_commit(drained);
         }
-        // the TMEM may go when every product issued has completed
-        commit(drained);
+        __syncwarp();
         if (!wait(drained, 0) && lane == 0)
             atomicOr(a.status, kStatusTimeout);
     } else {
@@ -394,20 +388,29 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         {
             unsigned char* q = q_sm + tile * kTileBytes;
             constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
-#pragma unroll 2
-            for (uint32_t i = 0; i < 32 / kAtOnce; ++i) {
-                const uint32_t in_warp = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
-                const uint32_t row = wrow + in_warp, tr = (warp % 4) * 32 + in_warp;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (row < rows) {
-                    const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + (int32_t)(row / a.group)) * a.q_token +
-                                 (int64_t)(kvh * a.group + row % a.group) * a.q_head + chunk * 8;
-                    if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0)
-                        w = *reinterpret_cast<const uint4*>(p);
-                    else
-                        w = make_uint4(load_pair<T>(p), load_pair<T>(p + 2), load_pair<T>(p + 4), load_pair<T>(p + 6));
+            const bool q_aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uint64_t)a.q_token * 2 | (uint64_t)a.q_head * 2) & 15u) == 0;
+            constexpr uint32_t kBatch = 8;  // loads in flight
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
+                uint4 w[kBatch];
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t row = wrow + (i0 + i) * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                    w[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row < rows) {
+                        const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + (int32_t)(row / a.group)) * a.q_token +
+                                     (int64_t)(kvh * a.group + row % a.group) * a.q_head + chunk * 8;
+                        if (q_aligned)
+                            w[i] = *reinterpret_cast<const uint4*>(p);
+                        else
+                            w[i] = load_row16<T>(p);
+                    }
                 }
-                *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w;
+#pragma unroll
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t tr = (warp % 4) * 32 + (i0 + i) * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                    *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w[i];
+                }
             }
             fence_proxy_async();
             __syncwarp();
@@ -422,40 +425,53 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         const float c = a.scale_log2;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
-        uint32_t t = 0;
-        for (; t < count; ++t) {
+#pragma unroll 1
+        for (uint32_t t = 0; t < count; ++t) {
             if (!(ok = wait(&s_ready[tile], t & 1)))
                 break;
             tc_fence_after();
-            const int32_t key0 = tiles.key(t);
-            const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
-            if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
-                // at the edges of what the rows see: hidden scores to -inf, in place
-#pragma unroll 1
-                for (int32_t i = 0; i < (int32_t)kPfKeys; i += 32) {
-                    uint32_t s[32];
-                    tmem_ld32(t_s + i, s);
-                    tmem_wait();
-                    const int32_t hi = pos - key0 - i, low = lo - key0 - i, sink = (int32_t)a.sinks - key0 - i;
-                    const uint32_t part = bits >> (i / 16);
-#pragma unroll
-                    for (int32_t e = 0; e < 32; ++e) {
-                        const bool seen = e <= hi && (e >= low || e < sink) && (part >> (e / 16) & 1u);
-                        s[e] = seen ? s[e] : 0xff800000u;
-                    }
-                    tmem_st32(t_s + i, s);
-                }
-                tmem_wait_st();
-            }
             uint32_t s[kPfKeys];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
                 tmem_ld32(t_s + i * 32, s + i * 32);
+            const int32_t key0 = tiles.key(t);
+            const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
+            if (tile == 0 && (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > tiles.last || key0 < tiles.lo)) {
+                // V rows that no row of this CTA sees become zeros before the first
+                // product with them (which waits for this tile's P)
+                const uint32_t slot = (2 * t + 1) % kStages;
+                if (!(ok = wait(&full[slot], ((2 * t + 1) / kStages) & 1)))
+                    break;
+                unsigned char* v = ring + slot * kTileBytes;
+#pragma unroll 1
+                for (uint32_t row = tid / 8; row < kPfKeys; row += 16) {
+                    const int32_t j = key0 + (int32_t)row;
+                    const bool used = (bits >> (row / 16) & 1u) && j <= tiles.last && (j >= tiles.lo || j < tiles.sink_end);
+                    if (!used)
+#pragma unroll
+                        for (uint32_t i = 0; i < kHalves; ++i)
+                            *reinterpret_cast<uint4*>(v + i * kHalfBytes + row * 128 + (lane % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async();
+            }
             tmem_wait();
+            if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
+                // at the edges of what the rows see: hidden scores to -inf
+                const int32_t hi = pos - key0, low = lo - key0, sink = (int32_t)a.sinks - key0;
+#pragma unroll
+                for (int32_t i = 0; i < (int32_t)kPfKeys; i += 32) {
+                    const uint32_t parts = bits >> (i / 16);
+                    const uint32_t seen = low_bits(hi - i + 1) & (~low_bits(low - i) | low_bits(sink - i)) &
+                                          ((parts & 1u ? 0xffffu : 0u) | (parts & 2u ? 0xffff0000u : 0u));
+#pragma unroll
+                    for (int32_t e = 0; e < 32; ++e)
+                        s[i + e] = seen & (1u << e) ? s[i + e] : 0xff800000u;
+                }
+            }
             float mx[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                mx[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 4]));
+            for (int e = 0; e < 4; ++e)
+                mx[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 4]));
 #pragma unroll
             for (int i = 8; i < (int)kPfKeys; i += 8)
 #pragma unroll
@@ -464,8 +480,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool grow = top > m && (top - m) * c > kSlack;  // also the first finite score
             if (__any_sync(0xffffffffu, grow)) {
-                const float mn = grow ? top : m;
-                const float w = grow ? exp2_fast((m - mn) * c) : 1.0f;
+                const float mn = grow ? top : m, w = grow ? exp2_fast((m - mn) * c) : 1.0f;
                 if (t > 0) {
                     // the product of the last keys has completed (s_ready)
 #pragma unroll 1
@@ -486,25 +501,26 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             const uint64_t c2 = f2_pack(c, c), n2 = f2_pack(neg, neg);
             uint64_t sum2[2] = {0, 0};
 #pragma unroll
-            for (uint32_t i = 0; i < kPfKeys; i += 64) {
+            for (uint32_t h = 0; h < 2; ++h) {
                 uint32_t p[32];
 #pragma unroll
-                for (uint32_t e = 0; e < 64; e += 2) {
-                    const uint64_t y = f2_fma((uint64_t)s[i + e] | ((uint64_t)s[i + e + 1] << 32), c2, n2);
-                    const float lo_p = exp2_fast(f2_lo(y)), hi_p = exp2_fast(f2_hi(y));
-                    sum2[(e / 2) & 1] = f2_add(sum2[(e / 2) & 1], f2_pack(lo_p, hi_p));
-                    p[e / 2] = pack2<T>(lo_p, hi_p);
+                for (uint32_t e = 0; e < kPfHalf; e += 2) {
+                    const uint32_t i = h * kPfHalf + e;
+                    const uint64_t y = f2_fma((uint64_t)s[i] | ((uint64_t)s[i + 1] << 32), c2, n2);
+                    const float w0 = exp2_fast(f2_lo(y)), w1 = exp2_fast(f2_hi(y));
+                    sum2[(e / 2) & 1] = f2_add(sum2[(e / 2) & 1], f2_pack(w0, w1));
+                    p[e / 2] = pack2<T>(w0, w1);
                 }
-                tmem_st32(t_s + i / 2, p);
+                tmem_st32(t_s + h * (kPfHalf / 2), p);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&p_ready[2 * tile + h]);
             }
             l += (f2_lo(sum2[0]) + f2_hi(sum2[0])) + (f2_lo(sum2[1]) + f2_hi(sum2[1]));
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(&p_ready[tile]);
         }
-        if (ok && count > 0)
+        if (ok && count > 0)  // every product is in O
             ok = wait(&s_ready[tile], count & 1);
         if (!ok && lane == 0)
             atomicOr(a.status, kStatusTimeout);
