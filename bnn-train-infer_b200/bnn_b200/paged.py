@@ -21,7 +21,7 @@ import ctypes
 import torch
 
 from . import _lib, accel
-from .accel import EINVAL, OK, BnnError
+from .accel import EINVAL, ENOTSUP, OK, BnnError
 
 try:
     from . import _paged_torch
@@ -36,7 +36,7 @@ def _bind():
     dll.bnn_b200_paged_sync.restype = ctypes.c_int
     dll.bnn_b200_paged_sync.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     dll.bnn_b200_paged_workspace.restype = ctypes.c_int
-    dll.bnn_b200_paged_workspace.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_size_t)]
+    dll.bnn_b200_paged_workspace.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_size_t)]
     dll.bnn_b200_device_ordinal.restype = ctypes.c_int
     dll.bnn_b200_device_ordinal.argtypes = [ctypes.c_void_p]
     return dll
@@ -48,16 +48,17 @@ class Paged:
     Calls on one stream run in order and share the workspace; a call on
     another stream first waits for the work the previous one had enqueued.
     A CUDA graph that captured a call uses the workspace too: replay it in
-    order with the other calls. max_batch and max_kv_heads bound the requests
-    and KV heads of a call (their product counts)."""
+    order with the other calls. max_batch: most requests of a call, a bound of
+    the program's own (calls beyond it are refused; the library's is 4096)."""
 
-    def __init__(self, device: accel.Device, max_batch=256, max_kv_heads=32):
+    def __init__(self, device: accel.Device, max_batch=4096):
         self._dll = _bind()
         self.device = device
         self._handle = device.handle.value
         self._index = self._dll.bnn_b200_device_ordinal(device.handle)
+        self._max_batch = max_batch
         need = ctypes.c_size_t()
-        st = self._dll.bnn_b200_paged_workspace(device.handle, max_batch, max_kv_heads, ctypes.byref(need))
+        st = self._dll.bnn_b200_paged_workspace(device.handle, ctypes.byref(need))
         if st != OK:
             raise BnnError(st, "bnn_b200_paged_workspace")
         self._workspace = torch.zeros(need.value, dtype=torch.uint8, device=f"cuda:{self._index}")
@@ -89,6 +90,8 @@ class Paged:
             f32 = out_dtype == torch.float32
             if not f32 and out_dtype != q.dtype or out is not None and out.dtype != out_dtype:
                 raise BnnError(EINVAL, "out_dtype: q's type or float32, and out's")
+        if page_table.shape[0] > self._max_batch:
+            raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
         raw = _paged_torch.stream(self._index)
         if raw != self._raw_stream:
             self._other_stream(raw)

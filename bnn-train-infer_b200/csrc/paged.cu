@@ -130,11 +130,12 @@ BNN_Status allow_smem(int ordinal, const void* kernel, size_t bytes) {
     return BNN_ENOTSUP;
 }
 
-// The workspace: for each CTA of the split kernel two records of partial rows
-// and two of joined groups; then two counters for each CTA and one for each
-// (request, KV head), zero between calls.
+// The workspace: for each CTA of the split kernel two records of partial rows,
+// two of joined groups and four counters, zero between calls.
 uint32_t split_grid(BNN_Device device) { return (uint32_t)device->sm_count * kDecPerSm; }
 size_t partial_bytes(BNN_Device device) { return (size_t)split_grid(device) * 4 * DecodeShape<128>::kRecord * sizeof(float); }
+
+size_t workspace_bytes(BNN_Device device) { return partial_bytes(device) + (size_t)split_grid(device) * 4 * sizeof(int); }
 
 template <int D, typename T>
 BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
@@ -144,7 +145,9 @@ BNN_Status launch_split(BNN_Device device, const AttnArgs& a, cudaStream_t strea
         return st;
     // no more CTAs than blocks there can be
     const uint64_t per_row = (((uint64_t)a.table_width << a.c.page_shift) + kDecBlock - 1) / kDecBlock + 1;
-    const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * (per_row + kRowCost);
+    const uint64_t groups = ((uint64_t)a.max_q * a.group + kDecRows - 1) / kDecRows;
+    const uint64_t most = (uint64_t)a.batch * a.c.kv_heads * (a.split_all ? groups : std::min(groups, (uint64_t)a.split_rows / kDecRows)) *
+                          (per_row + kRowCost);
     if (most > INT32_MAX)
         return BNN_ENOTSUP;  // the shares' units are counted in 32 bits
     return launch(attention_split_kernel<D, T>, dim3((uint32_t)std::min<uint64_t>(split_grid(device), most)), kDecThreads, smem,
@@ -200,13 +203,22 @@ BNN_Status launch_tiles(BNN_Device device, const AttnArgs& a, cudaStream_t strea
                   stream, args);
 }
 
+constexpr uint32_t kMixedCache = 1024;  // positions
+
 template <int D, typename T>
-BNN_Status attention_typed(BNN_Device device, const AttnArgs& a, cudaStream_t stream) {
-    // Requests of few rows go to the split kernel, the others to the tiles. One
-    // request is one kernel's, whatever its length.
-    if ((uint64_t)a.max_q * a.group <= kDecRows)
+BNN_Status attention_typed(BNN_Device device, AttnArgs a, cudaStream_t stream) {
+    // Requests of few rows go to the split kernel, the others to the tiles; each
+    // kernel finds its own. Where one of them can serve the whole call it goes
+    // alone (a launch that finds nothing to do costs 2 us): the split kernel if
+    // no request has more than 16 rows, the tiles if every cache is short (eight
+    // key tiles at most), either one for a single request.
+    const uint64_t most_rows = (uint64_t)a.max_q * a.group;
+    const bool long_cache = ((uint64_t)a.table_width << a.c.page_shift) >= kLongCache;
+    a.split_rows = kDecRows * std::max<uint32_t>(1, kSplitGroups / (a.c.kv_heads * std::min(a.batch, kSplitGroups)));
+    a.split_all = most_rows <= kDecRows || (long_cache && a.batch == 1 && most_rows <= a.split_rows);
+    if (a.split_all)
         return launch_split<D, T>(device, a, stream);
-    const bool mixed = a.batch > 1;
+    const bool mixed = a.batch > 1 && ((uint64_t)a.table_width << a.c.page_shift) >= kMixedCache;
     if (mixed) {
         const BNN_Status st = launch_split<D, T>(device, a, stream);
         if (st != BNN_OK)
@@ -299,10 +311,10 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
     return wide ? append_source<128, __half>(a, d.type, inter, s) : append_source<64, __half>(a, d.type, inter, s);
 }
 
-BNN_Status bnn_b200_paged_workspace(BNN_Device device, int64_t batch, int64_t kv_heads, size_t* bytes) {
-    if (!device || !bytes || batch <= 0 || batch > BNN_PAGED_MAX_BATCH || kv_heads <= 0 || kv_heads > 65536)
+BNN_Status bnn_b200_paged_workspace(BNN_Device device, size_t* bytes) {
+    if (!device || !bytes)
         return BNN_EINVAL;
-    *bytes = partial_bytes(device) + (((2 * (size_t)split_grid(device) + (size_t)batch * (size_t)kv_heads) * sizeof(int) + 255) & ~(size_t)255);
+    *bytes = workspace_bytes(device);
     return BNN_OK;
 }
 
@@ -332,11 +344,7 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
         return BNN_OK;
     if (!d.q || !d.out || (!d.page_table && d.table_width) || !d.kv_lens || !d.q_starts || !d.workspace)
         return BNN_EINVAL;
-    size_t need = 0;
-    st = bnn_b200_paged_workspace(device, d.batch, d.cache.kv_heads, &need);
-    if (st != BNN_OK)
-        return st;
-    if (d.workspace_bytes < 0 || (size_t)d.workspace_bytes < need || !aligned16(d.workspace))
+    if (d.workspace_bytes < 0 || (size_t)d.workspace_bytes < workspace_bytes(device) || !aligned16(d.workspace))
         return BNN_EINVAL;
     a.q = static_cast<const unsigned char*>(d.q);
     a.out = static_cast<unsigned char*>(d.out);

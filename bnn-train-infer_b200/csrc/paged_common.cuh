@@ -35,13 +35,15 @@ struct AttnArgs {
     const int32_t* q_starts;
     int64_t q_token, q_head, o_token, o_head, lse_token, table_stride;
     uint32_t batch, tokens, heads, group, table_width, max_q;
+    uint32_t split_rows;  // most rows of a request behind a long cache that the split kernel takes
+    uint32_t split_all;   // the split kernel takes every request
     uint32_t window, sinks;  // window 0: none
     uint32_t out_type;
     float scale;       // score scale
     float scale_log2;  // scale * log2(e)
     float* partials;   // workspace of the split kernel: records of partial rows
-    int* group_counters;
-    int* row_counters;
+    int* group_counters;  // two for each of the split kernel's CTAs, zero between calls
+    int* row_counters;    // the same
     int* status;
 };
 

@@ -37,6 +37,8 @@ constexpr uint32_t kMinShare = 4;                        // blocks
 // units of the time a block takes: shares are equal in blocks plus rows.
 constexpr uint32_t kRowCost = 3;
 constexpr uint32_t kDecRows = 16;
+constexpr uint32_t kLongCache = 2048;                    // positions
+constexpr uint32_t kSplitGroups = 128;                   // groups of 16 rows in a call (all requests and KV heads)
 constexpr uint32_t kJoin = 16;                           // parts of a row that one CTA joins at a time
 
 template <int D>
@@ -73,9 +75,20 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Request& r) {
     return s;
 }
 
-// This kernel's requests: those whose new tokens and heads fit the 16 rows.
+// This kernel's requests: those whose new tokens and heads fit the 16 rows, and
+// those behind a long cache whose rows make few enough groups of 16 (each group
+// reads the cache again, from L2 mostly). A tile's keys stay on one SM, here
+// they spread over all. 8 KV heads, group 2, tiles against groups: 24 tokens
+// behind 8192 positions 114 and 29 us, 100 tokens 115 and 69 us (104 groups),
+// 200 tokens 117 and 114 us; two requests of 64 behind 4000 60 and 52 us (128
+// groups), four 61 and 83 us; 100 behind 1000 22 and 25 us.
 __device__ __forceinline__ bool few_rows(const AttnArgs& a, const Request& r) {
-    return r.n > 0 && (uint32_t)r.n <= a.max_q && (uint32_t)r.n * a.group <= kDecRows;
+    const uint32_t rows = (uint32_t)r.n * a.group;
+    return r.n > 0 && (uint32_t)r.n <= a.max_q &&
+           (a.split_all || rows <= kDecRows || (rows <= a.split_rows && r.kv >= (int32_t)kLongCache));
+}
+__device__ __forceinline__ uint32_t row_groups(const AttnArgs& a, const Request& r) {
+    return ((uint32_t)r.n * a.group + kDecRows - 1) / kDecRows;
 }
 
 template <typename T>
@@ -134,24 +147,6 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int64_t at, const 
         store_out4_any<T>(a, at, x[0], x[1], x[2], x[3]);
 }
 
-// Scales and writes four values of one output row (and its lse with d == 0);
-// notes a row that is not finite.
-template <typename T>
-__device__ __noinline__ void finish4(const AttnArgs& a, uint32_t tok, uint32_t head, uint32_t d, float4 p, float sum, float mm,
-                                     uint32_t* odd_rows, uint32_t row) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float v[4] = {p.x * inv, p.y * inv, p.z * inv, p.w * inv};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = sum == 0.0f ? 0.0f : v[e];
-        if (!finite32(v[e]))
-            atomicOr(odd_rows, 1u << row);
-    }
-    store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
-    if (a.lse && d == 0)
-        a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, ln_fast(sum));
-}
-
 // Counts this CTA in: what its threads wrote before the barrier ahead of this
 // is visible to whoever counts last, and theirs to it.
 __device__ __forceinline__ int arrive(int* counter) {
@@ -160,15 +155,35 @@ __device__ __forceinline__ int arrive(int* counter) {
     return before;
 }
 
-// One stretch of a share: blocks [y0, y1) of row (b, kvh). The row's units begin
-// at row_begin, kRowCost of them before those of its blocks.
+// One stretch of a share: blocks [y0, y1) of row (b, kvh, group of 16 of the
+// matrix's rows from `first` on). The row's units begin at row_begin, kRowCost
+// of them before those of its blocks.
 struct Segment {
     Request r;
     Span sp;
-    uint32_t b, kvh, row_begin, y0, y1;
+    uint32_t b, kvh, first, row_begin, y0, y1;
     __device__ __forceinline__ uint32_t row_end() const { return row_begin + kRowCost + sp.count; }
     __device__ __forceinline__ uint32_t next() const { return row_begin + kRowCost + y1; }  // where its successor begins
 };
+
+// Scales and writes four values of one output row (and its lse with d == 0);
+// notes a row that is not finite.
+template <typename T>
+__device__ __noinline__ void finish4(const AttnArgs& a, const Segment& s, uint32_t in_group, uint32_t d, float4 p, float sum, float mm,
+                                     uint32_t* odd_rows, uint32_t bit) {
+    const uint32_t row = s.first + in_group, tok = (uint32_t)s.r.start + row / a.group, head = s.kvh * a.group + row % a.group;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float v[4] = {p.x * inv, p.y * inv, p.z * inv, p.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = sum == 0.0f ? 0.0f : v[e];
+        if (!finite32(v[e]))
+            atomicOr(odd_rows, 1u << bit);
+    }
+    store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
+    if (a.lse && d == 0)
+        a.lse[(int64_t)tok * a.lse_token + head] = sum == 0.0f ? -INFINITY : __fmaf_rn(mm, a.scale, ln_fast(sum));
+}
 
 // A row of which this CTA's share has a part: its shares c_first - 1 .. and so on.
 struct Cut {
@@ -209,7 +224,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             requests[b] = r;
             if (r.n > (int32_t)a.max_q && blockIdx.x == 0)
                 atomicOr(a.status, kPagedRange);
-            x = few_rows(a, r) ? (span_of(a, r).count + kRowCost) * a.c.kv_heads : 0;
+            x = few_rows(a, r) ? (span_of(a, r).count + kRowCost) * a.c.kv_heads * row_groups(a, r) : 0;
         }
         uint32_t sum = x;
 #pragma unroll
@@ -265,7 +280,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         const uint32_t at = raw_begin(blockIdx.x + i);
         uint32_t begin = at;
         if (at < total) {
-            const uint32_t b = request_at(at), len = (prefix[b + 1] - prefix[b]) / a.c.kv_heads, in = (at - prefix[b]) % len;
+            const uint32_t b = request_at(at), len = span_of(a, requests[b]).count + kRowCost, in = (at - prefix[b]) % len;
             begin = len > kWholeBlocks + kRowCost && in > kRowCost ? at : at - in;
         }
         ends[0] = i == 0 ? begin : ends[0];
@@ -280,8 +295,10 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         s.r = requests[s.b];
         s.sp = span_of(a, s.r);
         const uint32_t in = x - prefix[s.b], len = s.sp.count + kRowCost;
-        s.kvh = in / len;
-        const uint32_t y = in - s.kvh * len;
+        const uint32_t nth = in / len, groups = row_groups(a, s.r);
+        s.kvh = nth / groups;
+        s.first = (nth - s.kvh * groups) * kDecRows;
+        const uint32_t y = in - nth * len;
         s.row_begin = x - y;
         s.y0 = y > kRowCost ? y - kRowCost : 0;
         s.y1 = min(x_end - s.row_begin, len) - kRowCost;
@@ -361,7 +378,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
 #pragma unroll 1
                 for (uint32_t row = warp; row < kDecRows; row += kDecWarps)
                     if (odd >> row & 1u)
-                        attention_row<D, T>(a, s.b, s.r, (int32_t)(row / a.group), s.kvh * a.group + row % a.group);
+                        attention_row<D, T>(a, s.b, s.r, (int32_t)((s.first + row) / a.group), s.kvh * a.group + (s.first + row) % a.group);
             __syncthreads();
             if (tid == 0)
                 odd_rows &= (1u << first_bit) - 1u;
@@ -378,18 +395,18 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     while (x < x_end) {
         // ---- one segment
         const Segment s = segment_at(x);
-        const uint32_t nrows = (uint32_t)s.r.n * a.group;
+        const uint32_t nrows = min((uint32_t)s.r.n * a.group - s.first, kDecRows);
         // Q fragments: row i * group + head of the group
         uint32_t qf[D / 16][4];
         int32_t pos[2], lo[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint32_t row = g + half * 8, i = min(row / a.group, (uint32_t)s.r.n - 1);
+            const uint32_t row = s.first + g + half * 8, i = min(row / a.group, (uint32_t)s.r.n - 1);
             pos[half] = s.r.kv - s.r.n + (int32_t)i;
             lo[half] = window_begin(a, pos[half]);
             const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(s.r.start + (int32_t)i) * a.q_token +
                          (int64_t)(s.kvh * a.group + row % a.group) * a.q_head + t4 * 2;
-            const bool there = row < nrows;
+            const bool there = g + half * 8 < nrows;
             if ((reinterpret_cast<uintptr_t>(q) & 3u) == 0) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
@@ -405,6 +422,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 }
             }
         }
+        const int32_t first_pos = s.r.kv - s.r.n + (int32_t)(s.first / a.group);
+        const int32_t last_lo = window_begin(a, s.r.kv - s.r.n + (int32_t)((s.first + nrows - 1) / a.group));
         float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
@@ -444,8 +463,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                     sc[1][e] += odd[1][e];
                 }
             }
-            const bool inside = there && j0 + (int32_t)kDecTile - 1 <= s.r.kv - s.r.n &&
-                                (a.window == 0 || j0 > s.r.kv - 1 - (int32_t)a.window);
+            const bool inside = there && j0 + (int32_t)kDecTile - 1 <= first_pos && (a.window == 0 || j0 >= last_lo);
             if (!inside) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
@@ -551,7 +569,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 v.w = __fmaf_rn(p.w, e, v.w);
             }
             if (whole) {
-                finish4<T>(a, (uint32_t)s.r.start + row / a.group, s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows, row);
+                finish4<T>(a, s, row, d, v, sum, mm, &odd_rows, row);
             } else {
                 *reinterpret_cast<float4*>(record + 2 * kDecRows + row * D + d) = v;
                 if (d == 0) {
@@ -598,7 +616,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 const uint32_t n = round == 0 ? min(kJoin, k.parts - k.first_of_group)
                                    : grouped ? (k.parts + kJoin - 1) / kJoin : k.parts;
                 int* counter = round == 0 ? a.group_counters + k.place(k.first_of_group)
-                                          : a.row_counters + k.s.b * a.c.kv_heads + k.s.kvh;
+                                          : a.row_counters + k.place(0);
                 if (arrive(counter) == (int)n - 1) {
                     *counter = 0;  // as the next call expects it
                     k.n = n;
@@ -610,7 +628,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
 #pragma unroll 1
         for (uint32_t i = 0; i < cuts; ++i) {
             const Cut& k = cut[i];
-            const uint32_t n = k.n, nrows = (uint32_t)k.s.r.n * a.group;
+            const uint32_t n = k.n, nrows = min((uint32_t)k.s.r.n * a.group - k.s.first, kDecRows);
             if (n == 0)
                 continue;
             // record of the p-th of the n parts; the groups' lie behind the shares'
@@ -658,8 +676,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                     }
                 }
                 if (round == 1) {
-                    finish4<T>(a, (uint32_t)k.s.r.start + row / a.group, k.s.kvh * a.group + row % a.group, d, v, sum, mm, &odd_rows,
-                               row + 16 * i);
+                    finish4<T>(a, k.s, row, d, v, sum, mm, &odd_rows, row + kDecRows * i);
                 } else {
                     *reinterpret_cast<float4*>(joined + 2 * kDecRows + row * D + d) = v;
                     if (d == 0) {
@@ -672,7 +689,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     }
 #pragma unroll 1
     for (uint32_t i = 0; i < cuts; ++i)
-        redo(cut[i].s, 16 * i);
+        redo(cut[i].s, kDecRows * i);
 }
 
 }  // namespace paged

@@ -177,7 +177,8 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     uint32_t* mapped = reinterpret_cast<uint32_t*>(drained + 1);  // [16] bit u: 16-key part u of tile t (mod 16) is in memory
     uint32_t* tmem_slot = mapped + 16;
     __shared__ uint32_t warp_sum[32];
-    __shared__ uint32_t item_request, item_before;
+    __shared__ Request found;
+    __shared__ uint32_t found_item, found_request;
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     griddep_launch_dependents();
@@ -194,64 +195,69 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         }
         mbar_init(drained, 1);
         fence_barrier_init();
-        item_request = ~0u;
     }
     griddep_wait();
 
     // ---- which rows: items of kItemRows rows, request by request, heads side by
     // side; the last ones (they see the most keys of a prompt) first
-    uint32_t total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        const uint32_t mine = total;  // pass 1: the number of items
-        uint32_t seen = 0;
-        for (uint32_t b0 = 0; b0 < a.batch; b0 += Shape::kThreads) {
-            const uint32_t b = b0 + tid;
-            uint32_t x = 0;
-            if (b < a.batch) {
-                const Request r = load_request(a, b);
-                if (r.n > (int32_t)a.max_q) {
-                    if (blockIdx.x == 0)
-                        atomicOr(a.status, kPagedRange);
-                } else if (r.n > 0 && (args.every_request || !few_rows(a, r))) {
-                    x = ((uint32_t)r.n * a.group + kItemRows - 1) / kItemRows;
-                }
+    const uint32_t nth = blockIdx.x / a.c.kv_heads, kvh = blockIdx.x % a.c.kv_heads;
+    uint32_t total = 0, x = 0, at = 0;  // a thread's request: its items, those before it
+    Request mine = {};
+    auto scan = [&](uint32_t b, uint32_t seen) {
+        x = 0;
+        if (b < a.batch) {
+            mine = load_request(a, b);
+            if (mine.n > (int32_t)a.max_q) {
+                if (blockIdx.x == 0)
+                    atomicOr(a.status, kPagedRange);
+            } else if (mine.n > 0 && (args.every_request || !few_rows(a, mine))) {
+                x = ((uint32_t)mine.n * a.group + kItemRows - 1) / kItemRows;
             }
-            uint32_t sum = x;
+        }
+        uint32_t sum = x;
 #pragma unroll
-            for (uint32_t d = 1; d < 32; d <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
-                sum += lane >= d ? y : 0;
-            }
-            if (lane == 31)
-                warp_sum[warp] = sum;
+        for (uint32_t d = 1; d < 32; d <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, sum, d);
+            sum += lane >= d ? y : 0;
+        }
+        if (lane == 31)
+            warp_sum[warp] = sum;
+        __syncthreads();
+        at = seen + sum - x;
+        for (uint32_t w = 0; w < Shape::kThreads / 32; ++w) {
+            at += w < warp ? warp_sum[w] : 0;
+            seen += warp_sum[w];
+        }
+        return seen;
+    };
+#pragma unroll 1
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += Shape::kThreads) {
+        total = scan(b0 + tid, total);
+        if (a.batch > Shape::kThreads)
             __syncthreads();
-            uint32_t before = seen;
-            for (uint32_t w = 0; w < Shape::kThreads / 32; ++w) {
-                before += w < warp ? warp_sum[w] : 0;
-                seen += warp_sum[w];
-            }
-            if (pass == 1) {
-                const uint32_t item = mine - 1 - blockIdx.x / a.c.kv_heads;
-                const uint32_t at = before + sum - x;
-                if (item >= at && item < at + x) {
-                    item_request = b;
-                    item_before = at;
-                }
-            }
+    }
+    if (nth >= total)
+        return;
+    const uint32_t item = total - 1 - nth;
+    uint32_t request = tid;
+    auto claim = [&]() {
+        if (item - at < x) {  // exactly one thread's
+            found = mine;
+            found_item = item - at;
+            found_request = request;
+        }
+    };
+    if (a.batch <= Shape::kThreads) {
+        claim();
+    } else {
+        uint32_t seen = 0;
+#pragma unroll 1
+        for (request = tid; request - tid < a.batch; request += Shape::kThreads) {
+            seen = scan(request, seen);
+            claim();
             __syncthreads();
         }
-        total = seen;
-        if (pass == 0 && blockIdx.x / a.c.kv_heads >= total)
-            return;
     }
-    const uint32_t b = item_request, kvh = blockIdx.x % a.c.kv_heads;
-    const Request r = load_request(a, b);
-    const uint32_t row0 = (total - 1 - blockIdx.x / a.c.kv_heads - item_before) * kItemRows;
-    const uint32_t rows = (uint32_t)r.n * a.group;
-    const int32_t base_pos = r.kv - r.n;
-    const KeyTiles tiles = key_tiles(a, base_pos + (int32_t)(row0 / a.group),
-                                     base_pos + (int32_t)(min(row0 + kItemRows, rows) - 1) / (int32_t)a.group);
-    const uint32_t count = tiles.count;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                      "r"(Shape::kTmemCols));
@@ -260,6 +266,14 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const uint32_t b = found_request;
+    const Request r = found;
+    const uint32_t row0 = found_item * kItemRows;
+    const uint32_t rows = (uint32_t)r.n * a.group;
+    const int32_t base_pos = r.kv - r.n;
+    const KeyTiles tiles = key_tiles(a, base_pos + (int32_t)(row0 / a.group),
+                                     base_pos + (int32_t)(min(row0 + kItemRows, rows) - 1) / (int32_t)a.group);
+    const uint32_t count = tiles.count;
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + kTiles * kPfKeys;
 

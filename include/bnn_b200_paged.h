@@ -125,8 +125,8 @@ typedef struct {
 } BNN_PagedAttention;
 BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention* desc, void* stream);
 
-/* Workspace of calls of at most `batch` requests and `kv_heads` KV heads. */
-BNN_Status bnn_b200_paged_workspace(BNN_Device device, int64_t batch, int64_t kv_heads, size_t* bytes);
+/* Bytes of the workspace (the device's size alone decides: about 20 MB). */
+BNN_Status bnn_b200_paged_workspace(BNN_Device device, size_t* bytes);
 
 /* Waits for `stream` and returns what the paged calls of this handle recorded
  * since the last one: BNN_ERANGE (see above), BNN_ETIMEOUT (a bounded device

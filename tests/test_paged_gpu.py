@@ -152,6 +152,17 @@ def test_a_few_new_tokens(ops, requests, group):
     check(ops, make(requests, 2 * group, 2, 64, 32, F16), window=40, sinks=2)
 
 
+@pytest.mark.parametrize("requests,window,sinks", [
+    ([(100, 3000)], 0, 0), ([(9, 1024)], 0, 0), ([(120, 1500)], 200, 5), ([(40, 2100)], 1500, 0),  # one request: its rows in groups of 16
+    ([(20, 1024), (20, 1023), (1, 4000), (300, 1500), (17, 2500)], 0, 0),  # some of each kernel's
+    ([(30, 1800), (200, 1900), (64, 64), (2, 1100)], 300, 20), ([(33, 1200), (0, 0), (5, 0)], 0, 0)])
+@pytest.mark.parametrize("d,hq,hkv,page,dtype", [(128, 4, 2, 16, BF16), (64, 8, 1, 64, F16), (128, 5, 1, 32, F16)])
+def test_groups_of_rows_behind_a_long_cache(ops, requests, window, sinks, d, hq, hkv, page, dtype):
+    check(ops, make(requests, hq, hkv, d, page, dtype), window=window, sinks=sinks)
+    check(ops, make(requests, hq, hkv, d, page, dtype, junk=math.nan, window=window, sinks=sinks, released=bool(window)), window=window,
+          sinks=sinks)
+
+
 @pytest.mark.parametrize("junk", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("requests,window,sinks", [([(1, 37), (1, 300), (1, 129)], 0, 0), ([(1, 500), (1, 33)], 70, 3),
                                                    ([(40, 140), (130, 500)], 0, 0), ([(40, 700), (130, 400)], 70, 3)])
@@ -482,13 +493,18 @@ def test_more_new_tokens_than_declared(ops):
             within(out[n:], want[n:], tol[n:])
 
 
-def test_workspace_too_small(ops):
+def test_workspace_too_small_and_too_many_requests(ops):
     from bnn_b200 import accel, paged
-    little = paged.Paged(ops.device, max_batch=1, max_kv_heads=1)
-    made = make([(1, 20)] * 300, 64, 32, 64, 16, BF16)
+    made = make([(1, 20)] * 3, 4, 2, 64, 16, BF16)
+    small = paged.Paged(ops.device, max_batch=3)
+    check(small, made)
+    small._workspace = small._workspace[:-1]
     with pytest.raises(accel.BnnError) as e:
-        little.attention(*made, max_q=1)
+        small.attention(*made, max_q=1)
     assert e.value.status == accel.EINVAL
+    with pytest.raises(accel.BnnError) as e:
+        paged.Paged(ops.device, max_batch=2).attention(*made, max_q=1)
+    assert e.value.status == accel.ENOTSUP
 
 
 def test_append_refusals(ops):
@@ -547,3 +563,13 @@ def test_starved_loads_time_out_then_recover(ops):
         assert hook(ops.device.handle, 0, 0) == accel.OK
     assert e.value.status == accel.ETIMEOUT
     check(ops, made)
+
+
+@pytest.mark.parametrize("batch", [127, 320, 321, 1000])
+def test_many_requests(ops, batch):
+    """More requests than a CTA has threads, of all sizes."""
+    r = random.Random(batch)
+    few = [(r.choice((0, 1, 1, 1, 2)), r.randrange(0, 90)) for _ in range(batch)]
+    check(ops, make(few, 2, 1, 64, 16, BF16))
+    some = [(r.choice((0, 1, 1, 9, 40)), r.randrange(0, 90)) for _ in range(batch - 1)] + [(150, 1200)]
+    check(ops, make(some, 2, 1, 64, 16, BF16))

@@ -18,7 +18,7 @@ def test_no_handle_is_refused(name):
     assert fn(None, None, None) == accel.EINVAL
     dll = paged._bind()
     assert dll.bnn_b200_paged_sync(None, None) == accel.EINVAL
-    assert dll.bnn_b200_paged_workspace(None, 1, 1, ctypes.byref(ctypes.c_size_t())) == accel.EINVAL
+    assert dll.bnn_b200_paged_workspace(None, ctypes.byref(ctypes.c_size_t())) == accel.EINVAL
 
 
 def test_host_tensors_are_refused():
