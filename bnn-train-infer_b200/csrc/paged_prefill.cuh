@@ -40,9 +40,14 @@ struct PrefillShape {
     static constexpr uint32_t kThreads = kTiles * 128 + 64;
     static constexpr uint32_t kTileBytes = kPfKeys * D * 2;  // of K, V or Q
     static constexpr uint32_t kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 4 : 8);
-    static constexpr uint32_t kTmemUsed = kTiles * (kPfKeys + D);
+    // 64-wide heads leave TMEM room for P beside S: then Q K^T of the next keys
+    // follows as soon as S is in registers, and the softmax need not wait for it
+    // (window chunks 198 -> 178 us). 128-wide heads fill the TMEM with S and O, and
+    // P takes S's place.
+    static constexpr bool kApart = D == 64;
+    static constexpr uint32_t kTmemUsed = kTiles * (kPfKeys + D + (kApart ? kPfHalf : 0));
     static constexpr uint32_t kTmemCols = kTmemUsed <= 256 ? 256 : 512;
-    static constexpr uint32_t kBars = 2 * kStages + 4 * kTiles + 1;
+    static constexpr uint32_t kBars = 2 * kStages + 6 * kTiles + 1;
     static constexpr size_t kSmem = 1024 + (size_t)(kTiles + kStages) * kTileBytes + kBars * 8 + 16 * 4 + 64;
 };
 
@@ -162,6 +167,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     constexpr uint32_t kHalfBytes = kPfKeys * 128;      // 16 KB
     constexpr uint32_t kLoadWarp = kTiles * 4, kMmaWarp = kTiles * 4 + 1;
     constexpr uint32_t kItemRows = kTiles * kPfRows;
+    constexpr bool kApart = Shape::kApart;
     const AttnArgs& a = args.a;
     extern __shared__ __align__(1024) unsigned char pf_smem[];
     const uint32_t raw = smem_addr(pf_smem);
@@ -173,7 +179,9 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     uint64_t* q_ready = empty + kStages;     // [kTiles] Q in shared memory
     uint64_t* s_ready = q_ready + kTiles;    // [kTiles] S in TMEM and the last keys' P V done
     uint64_t* p_ready = s_ready + kTiles;    // [kTiles][2] half of P in TMEM, O scaled
-    uint64_t* drained = p_ready + 2 * kTiles;
+    uint64_t* s_free = p_ready + 2 * kTiles;  // [kTiles] S in registers (kApart)
+    uint64_t* o_ready = s_free + kTiles;      // [kTiles] P V done (kApart)
+    uint64_t* drained = o_ready + kTiles;
     uint32_t* mapped = reinterpret_cast<uint32_t*>(drained + 1);  // [16] bit u: 16-key part u of tile t (mod 16) is in memory
     uint32_t* tmem_slot = mapped + 16;
     __shared__ uint32_t warp_sum[32];
@@ -192,6 +200,8 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             mbar_init(&s_ready[t], 1);
             mbar_init(&p_ready[2 * t], 4);
             mbar_init(&p_ready[2 * t + 1], 4);
+            mbar_init(&s_free[t], 4);
+            mbar_init(&o_ready[t], 1);
         }
         mbar_init(drained, 1);
         fence_barrier_init();
@@ -276,6 +286,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
     const uint32_t count = tiles.count;
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_o = tmem + kTiles * kPfKeys;
+    const uint32_t tmem_p = kApart ? tmem_o + kTiles * D : tmem, p_step = kApart ? kPfHalf : kPfKeys;  // tile's P
 
     if (warp == kLoadWarp) {
         // ---- K and V tiles, page by page: lane p has the tile's p-th page
@@ -362,6 +373,20 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
 #pragma unroll 1
                 for (uint32_t t = 0; ok && t < count; ++t) {
                     const bool more = t + 1 < count;
+                    auto next_scores = [&](uint32_t tile) {
+                        if (more && (tile != 0 || need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0))))
+                            qk(tile, t + 1);
+                        if (more && tile == kTiles - 1)
+                            mma_commit(&empty[slot_of(t + 1, 0)]);
+                    };
+                    if constexpr (kApart) {
+#pragma unroll 1
+                        for (uint32_t tile = 0; more && tile < kTiles && need(&s_free[tile], t & 1); ++tile) {
+                            tc_fence_after();
+                            next_scores(tile);
+                            mma_commit(&s_ready[tile]);
+                        }
+                    }
                     if (!need(&full[slot_of(t, 1)], parity_of(t, 1)))
                         break;
                     const uint64_t va = v_desc + (slot_of(t, 1) * kTileBytes >> 4);
@@ -372,18 +397,19 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                             tc_fence_after();
 #pragma unroll
                             for (uint32_t k = 0; k < kPfHalf / 16; ++k)
-                                mma_f16_ts(tmem_o + tile * D, tmem + tile * kPfKeys + h * (kPfHalf / 2) + k * 8,
+                                mma_f16_ts(tmem_o + tile * D, tmem_p + tile * p_step + h * (kPfHalf / 2) + k * 8,
                                            va + ((h * kPfHalf + k * 16) * 128 >> 4), kPvDesc, t != 0 || h != 0 || k != 0);
                         }
-                        if (!ok || (more && tile == 0 && !need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0))))
+                        if (!ok)
                             break;
-                        if (more)
-                            qk(tile, t + 1);
-                        mma_commit(&s_ready[tile]);
+                        if constexpr (kApart) {
+                            mma_commit(&o_ready[tile]);
+                        } else {
+                            next_scores(tile);
+                            mma_commit(&s_ready[tile]);
+                        }
                     }
                     mma_commit(&empty[slot_of(t, 1)]);
-                    if (more)
-                        mma_commit(&empty[slot_of(t + 1, 0)]);
                 }
             }
             if (!ok)
@@ -399,11 +425,12 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         const uint32_t tile = warp / 4, wrow = row0 + tile * kPfRows + (warp % 4) * 32;  // the warp's first row
         const uint32_t lane_off = ((warp % 4) * 32u) << 16;
         const uint32_t t_s = tmem + tile * kPfKeys + lane_off, t_o = tmem_o + tile * D + lane_off;
+        const uint32_t t_p = tmem_p + tile * p_step + lane_off;
         {
             unsigned char* q = q_sm + tile * kTileBytes;
             constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
             const bool q_aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uint64_t)a.q_token * 2 | (uint64_t)a.q_head * 2) & 15u) == 0;
-            constexpr uint32_t kBatch = 8;  // loads in flight
+            constexpr uint32_t kBatch = 32 / kAtOnce;  // loads in flight: all of the warp's
 #pragma unroll 1
             for (uint32_t i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
                 uint4 w[kBatch];
@@ -469,6 +496,12 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 fence_proxy_async();
             }
             tmem_wait();
+            if constexpr (kApart) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&s_free[tile]);
+            }
             if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
                 // at the edges of what the rows see: hidden scores to -inf
                 const int32_t hi = pos - key0, low = lo - key0, sink = (int32_t)a.sinks - key0;
@@ -493,10 +526,16 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                     mx[e] = max3(mx[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + e + 4]));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const bool grow = top > m && (top - m) * c > kSlack;  // also the first finite score
+            if constexpr (kApart) {
+                // the last keys' product has read P and is in O
+                if (t > 0 && !(ok = wait(&o_ready[tile], (t - 1) & 1)))
+                    break;
+                tc_fence_after();
+            }
             if (__any_sync(0xffffffffu, grow)) {
                 const float mn = grow ? top : m, w = grow ? exp2_fast((m - mn) * c) : 1.0f;
                 if (t > 0) {
-                    // the product of the last keys has completed (s_ready)
+                    // the product of the last keys has completed (s_ready, o_ready)
 #pragma unroll 1
                     for (uint32_t i = 0; i < D / 32; ++i) {
                         uint32_t o[32];
@@ -525,7 +564,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                     sum2[(e / 2) & 1] = f2_add(sum2[(e / 2) & 1], f2_pack(w0, w1));
                     p[e / 2] = pack2<T>(w0, w1);
                 }
-                tmem_st32(t_s + h * (kPfHalf / 2), p);
+                tmem_st32(t_p + h * (kPfHalf / 2), p);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -535,7 +574,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             l += (f2_lo(sum2[0]) + f2_hi(sum2[0])) + (f2_lo(sum2[1]) + f2_hi(sum2[1]));
         }
         if (ok && count > 0)  // every product is in O
-            ok = wait(&s_ready[tile], count & 1);
+            ok = kApart ? wait(&o_ready[tile], (count - 1) & 1) : wait(&s_ready[tile], count & 1);
         if (!ok && lane == 0)
             atomicOr(a.status, kStatusTimeout);
         if (ok) {
