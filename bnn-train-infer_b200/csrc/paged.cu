@@ -65,6 +65,15 @@ BNN_Status launch(void (*kernel)(Args), dim3 grid, uint32_t threads, size_t smem
     return BNN_OK;
 }
 
+// The kernels here let their successor start early, and a one-row BNN job may
+// read its input before it waits for its predecessor (GemvArgs::early_input):
+// on the handle's own stream it must not while a paged call's outputs are in
+// flight.
+void outputs_in_flight(BNN_Device device, cudaStream_t stream) {
+    if (stream == device->stream)
+        device->inflight_overflow = true;
+}
+
 // ---- append
 
 constexpr uint64_t kAppendWide = 148 * 64;  // (token, head) rows: more than the warps that fit the GPU at once
@@ -305,6 +314,7 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
         return BNN_EIO;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = d.cache.head_dim == 128, inter = d.interleaved != 0;
+    outputs_in_flight(device, s);
     if (d.cache.type == BNN_PAGED_BF16)
         return wide ? append_source<128, __nv_bfloat16>(a, d.type, inter, s)
                     : append_source<64, __nv_bfloat16>(a, d.type, inter, s);
@@ -378,6 +388,7 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
         return BNN_EIO;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = d.cache.head_dim == 128;
+    outputs_in_flight(device, s);
     if (d.cache.type == BNN_PAGED_BF16)
         return wide ? attention_typed<128, __nv_bfloat16>(device, a, s) : attention_typed<64, __nv_bfloat16>(device, a, s);
     return wide ? attention_typed<128, __half>(device, a, s) : attention_typed<64, __half>(device, a, s);
