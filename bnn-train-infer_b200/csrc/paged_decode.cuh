@@ -188,7 +188,8 @@ __device__ __noinline__ void finish4(const AttnArgs& a, const Segment& s, uint32
 // A row of which this CTA's share has a part: its shares c_first - 1 .. and so on.
 struct Cut {
     Segment s;
-    uint32_t c_first, parts, first_of_group, level, n;
+    uint32_t c_first, parts, first_of_group, n;
+    bool joins_group;
     // where the p-th part, or the group that begins with it, has its record: a
     // share ends one cut row (0) and begins another (1) at most
     __device__ __forceinline__ uint32_t place(uint32_t p) const { return 2 * (c_first - 1 + p) + (p == 0 ? 1u : 0u); }
@@ -258,16 +259,17 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         return;
     const uint32_t even = total / shares, extra = total % shares;  // the first `extra` shares have one unit more
 
-    // the request that unit x belongs to
+    // the request that unit x belongs to (all lanes of a warp ask for the same x:
+    // 32 prefixes a look)
+    uint32_t widest = 1;
+    while (widest * 32 < a.batch)
+        widest *= 32;
     auto request_at = [&](uint32_t x) {
-        uint32_t lo = 0, hi = a.batch;
+        uint32_t lo = 0;
 #pragma unroll 1
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (prefix[mid] <= x)
-                lo = mid;
-            else
-                hi = mid;
+        for (uint32_t step = widest; step; step /= 32) {
+            const uint32_t b = lo + lane * step;
+            lo += (__popc(__ballot_sync(0xffffffffu, b < a.batch && prefix[b] <= x)) - 1) * step;
         }
         return lo;
     };
@@ -391,7 +393,8 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         return at < cut ? at / (even + 1) : extra + (at - cut) / even;
     };
 
-    uint32_t x = x_begin, slot = 0, cuts = 0, cut_x[2] = {0, 0};
+    uint32_t x = x_begin, slot = 0, cuts = 0;
+    bool grouped = false;  // one of the cut rows has more than kJoin parts
     while (x < x_end) {
         // ---- one segment
         const Segment s = segment_at(x);
@@ -545,6 +548,15 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         // shares that begin behind this row's first block: c_first .. c_last
         const uint32_t c_first = share_of(s.row_begin + kRowCost) + 1, c_last = share_of(s.row_end() - 1);
         const bool whole = s.sp.count <= kWholeBlocks || c_first > c_last;
+        if (!whole && tid == 0) {
+            // at most two: the row that an earlier share began, and the last one
+            Cut& k = cut[cuts];
+            k.s = s;
+            k.c_first = c_first;
+            k.parts = c_last - c_first + 2;
+            k.first_of_group = (blockIdx.x - (c_first - 1)) / kJoin * kJoin;
+            k.joins_group = false;
+        }
         // the record of this share's part of a cut row: 1 if the row begins in this share, else 0
         float* record = a.partials + (2ull * blockIdx.x + (s.y0 != 0 ? 0u : 1u)) * Shape::kRecord;
 
@@ -578,13 +590,12 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                 }
             }
         }
-        if (!whole) {
-            // at most two: the row that an earlier share began, and the last one
-            cut_x[cuts == 0 ? 0 : 1] = x;
-            ++cuts;
-            __syncthreads();
-        } else {
+        if (whole) {
             redo(s, 0);
+        } else {
+            ++cuts;
+            grouped |= c_last - c_first + 2 > kJoin;
+            __syncthreads();
         }
         x = s.next();
     }
@@ -596,31 +607,21 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     // arrives when all its work is done: the joint sums hold up no stream.
     if (cuts == 0)
         return;
-    if (tid < cuts) {
-        const Segment c = segment_at(cut_x[tid]);
-        Cut& k = cut[tid];
-        k.s = c;
-        k.c_first = share_of(c.row_begin + kRowCost) + 1;
-        k.parts = share_of(c.row_end() - 1) - k.c_first + 2;
-        k.first_of_group = (blockIdx.x - (k.c_first - 1)) / kJoin * kJoin;
-        k.level = k.parts > kJoin ? 0 : 1;
-    }
 #pragma unroll 1
-    for (uint32_t round = 0; round < 2; ++round) {
+    for (uint32_t round = grouped ? 0 : 1; round < 2; ++round) {
         __syncthreads();  // the CTA's records are written
         if (tid < cuts) {
             Cut& k = cut[tid];
+            const bool in_groups = k.parts > kJoin;
             k.n = 0;
-            if (k.level == round || (round == 1 && k.level == 2)) {
-                const bool grouped = k.parts > kJoin;
+            if (round == 0 ? in_groups : !in_groups || k.joins_group) {
                 const uint32_t n = round == 0 ? min(kJoin, k.parts - k.first_of_group)
-                                   : grouped ? (k.parts + kJoin - 1) / kJoin : k.parts;
-                int* counter = round == 0 ? a.group_counters + k.place(k.first_of_group)
-                                          : a.row_counters + k.place(0);
+                                   : in_groups ? (k.parts + kJoin - 1) / kJoin : k.parts;
+                int* counter = round == 0 ? a.group_counters + k.place(k.first_of_group) : a.row_counters + k.place(0);
                 if (arrive(counter) == (int)n - 1) {
                     *counter = 0;  // as the next call expects it
                     k.n = n;
-                    k.level = round == 0 ? 2 : k.level;  // 2: this CTA joined the group and counts for it
+                    k.joins_group = round == 0;  // this CTA has joined the group and counts for it
                 }
             }
         }
@@ -632,9 +633,9 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
             if (n == 0)
                 continue;
             // record of the p-th of the n parts; the groups' lie behind the shares'
-            const bool grouped = round == 1 && k.parts > kJoin;
-            const uint32_t p_begin = round == 0 ? k.first_of_group : 0, p_step = grouped ? kJoin : 1;
-            const float* records = a.partials + (grouped ? 2ull * gridDim.x * Shape::kRecord : 0ull);
+            const bool of_groups = round == 1 && k.parts > kJoin;
+            const uint32_t p_begin = round == 0 ? k.first_of_group : 0, p_step = of_groups ? kJoin : 1;
+            const float* records = a.partials + (of_groups ? 2ull * gridDim.x * Shape::kRecord : 0ull);
             float* joined = a.partials + (2ull * gridDim.x + k.place(k.first_of_group)) * Shape::kRecord;
             // both rows at once where there are two and threads for them
             const uint32_t quads = nrows * (D / 4);
