@@ -7,6 +7,11 @@
 // converted. A head is D / 4 lanes of a warp, four adjacent values each, so
 // the mean is a butterfly over those lanes, and the other value of a pair
 // (i, i + rotary / 2) is rotary / 8 lanes away (adjacent pairs: in the lane).
+//
+// Bound: HBM for long calls (8192 tokens of 32 heads from FP32, 206 MB, 35.7 us
+// = 5.8 TB/s, 88% of the measured copy rate; instruction issue 57% busy, before
+// the heads of a warp were of one kind it was the limit at 53 us), the launch
+// for short ones.
 #pragma once
 
 #include "paged_common.cuh"

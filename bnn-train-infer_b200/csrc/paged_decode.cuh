@@ -26,20 +26,25 @@
 namespace bnn {
 namespace paged {
 
+// Measured on a B200 (copy rate 6.54 TB/s): 2 requests of 131071 positions,
+// 1.07 GB, 167 us = 6.4 TB/s; 8 of 4096 29.4 us, of which 5 us pass until the
+// first keys are in (lengths, then page numbers, then keys: three dependent
+// reads) and 4 us in the joins; 61 of 1 to 16384 75 us; one of 160 8 us.
 constexpr uint32_t kDecWarps = 4;
 constexpr uint32_t kDecThreads = kDecWarps * 32;
-constexpr uint32_t kDecTile = 16;                        // keys of a warp's step
-constexpr uint32_t kDecBlock = kDecTile * kDecWarps;     // keys of a CTA's step
-constexpr uint32_t kDecPerSm = 2;                        // CTAs an SM holds
-constexpr uint32_t kWholeBlocks = 8;
-constexpr uint32_t kMinShare = 4;                        // blocks
+constexpr uint32_t kDecTile = 16;                     // keys of a warp's step
+constexpr uint32_t kDecBlock = kDecTile * kDecWarps;  // keys of a CTA's step
+constexpr uint32_t kDecPerSm = 2;                     // CTAs an SM holds: 192 KB of ring
+constexpr uint32_t kWholeBlocks = 8;                  // a join costs as much as these blocks
+constexpr uint32_t kMinShare = 4;                     // units (below)
 // A row's fixed work (its queries, the pipeline's start, the joint sum) in
-// units of the time a block takes: shares are equal in blocks plus rows.
+// units of the time a block takes: shares are equal in blocks plus rows (61
+// ragged requests: 132 us with 0, 78 with 2, 73 with 3 on the same code).
 constexpr uint32_t kRowCost = 3;
 constexpr uint32_t kDecRows = 16;
-constexpr uint32_t kLongCache = 2048;                    // positions
-constexpr uint32_t kSplitGroups = 128;                   // groups of 16 rows in a call (all requests and KV heads)
-constexpr uint32_t kJoin = 16;                           // parts of a row that one CTA joins at a time
+constexpr uint32_t kLongCache = 2048;   // positions
+constexpr uint32_t kSplitGroups = 128;  // groups of 16 rows in a call (all requests and KV heads)
+constexpr uint32_t kJoin = 16;          // parts of a row that one CTA joins at a time
 
 template <int D>
 struct DecodeShape {
@@ -48,7 +53,7 @@ struct DecodeShape {
     static constexpr uint32_t kWarpBytes = kStages * kStageBytes;
     static constexpr uint32_t kRingBytes = kDecWarps * kWarpBytes;
     static constexpr uint32_t kRecord = kDecRows * (D + 2);  // floats of a partial: m[16], l[16], O[16][D]
-    static_assert(kDecRows * D * 4 <= kWarpBytes, "a warp's O fits its ring");
+    static_assert(kDecRows * D * 4 <= kStageBytes, "a warp's O fits a stage");
 };
 
 inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * (4 + sizeof(Request)); }

@@ -19,6 +19,19 @@
 // 128-key tiles. A position that no row of the CTA sees may hold anything:
 // its scores are replaced, and its V row is overwritten with zeros before
 // the product.
+//
+// Bound: the chain S -> softmax -> P -> products -> S of a tile. Of 3850 clocks
+// that a step of 128 keys takes for both row tiles (8192 tokens, 295 us,
+// 0.93 PFLOP/s at the 1.7 GHz that the tensor cores leave) a tile's softmax
+// works 2450 (exponentials 1420: 128 a row at 16 a clock and SM are 1024) and
+// waits 1400 for products and hand-overs; MUFU and tensor pipe are each busy
+// half of the time. The TMEM holds S and O of two tiles of 128-wide heads and no
+// more, so a third chain, or a second S, has no room. Tried and slower: steps of
+// 64 keys with two S buffers (products 64 wide take 53 clocks instead of half of
+// 65: 333 us), exponentials on the FMA pipe for a quarter to a half of the
+// weights (303 to 316 us: five FMAs of two values cost what they save), weights
+// taken with the old maximum (367 us), products in the order in which weights
+// arrive (322 us), weights handed over all at once (306 us).
 #pragma once
 
 #include <cuda.h>

@@ -65,7 +65,8 @@ typedef struct {
  * up to head_dim. A position outside the table leaves the token's q_out rows
  * zero and stores nothing, a slot outside the cache stores nothing; both make
  * the next bnn_b200_paged_sync return BNN_ERANGE. Two tokens of one call
- * must not share a slot. */
+ * must not share a slot. q_out's rows lie on 8-byte boundaries; q, k and v may
+ * lie anywhere (16-byte rows load faster). */
 typedef struct {
     BNN_PagedCache cache;
     const void* q;
