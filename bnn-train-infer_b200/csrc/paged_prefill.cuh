@@ -443,28 +443,38 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             unsigned char* q = q_sm + tile * kTileBytes;
             constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
             const bool q_aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uint64_t)a.q_token * 2 | (uint64_t)a.q_head * 2) & 15u) == 0;
-            constexpr uint32_t kBatch = 32 / kAtOnce;  // loads in flight: all of the warp's
-#pragma unroll 1
-            for (uint32_t i0 = 0; i0 < 32 / kAtOnce; i0 += kBatch) {
-                uint4 w[kBatch];
+            constexpr uint32_t kLoads = 32 / kAtOnce;
+            const uint32_t chunk = lane % kChunks;
+            uint32_t row = wrow + lane / kChunks, tok = row / a.group, head = row % a.group;
+            const T* base = reinterpret_cast<const T*>(a.q) + (int64_t)r.start * a.q_token + (int64_t)(kvh * a.group) * a.q_head + chunk * 8;
+            uint4 w[kLoads];
+            // all of the warp's rows at once, nothing between the loads that would
+            // make one wait for another
+            if (q_aligned) {
 #pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i) {
-                    const uint32_t row = wrow + (i0 + i) * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                for (uint32_t i = 0; i < kLoads; ++i) {
                     w[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < rows) {
-                        const T* p = reinterpret_cast<const T*>(a.q) + (int64_t)(r.start + (int32_t)(row / a.group)) * a.q_token +
-                                     (int64_t)(kvh * a.group + row % a.group) * a.q_head + chunk * 8;
-                        if (q_aligned)
-                            w[i] = *reinterpret_cast<const uint4*>(p);
-                        else
-                            w[i] = load_row16<T>(p);
-                    }
+                    if (row < rows)
+                        w[i] = *reinterpret_cast<const uint4*>(base + (int64_t)tok * a.q_token + (int64_t)head * a.q_head);
+                    row += kAtOnce;
+                    for (head += kAtOnce; head >= a.group; head -= a.group)
+                        ++tok;
                 }
+            } else {
 #pragma unroll
-                for (uint32_t i = 0; i < kBatch; ++i) {
-                    const uint32_t tr = (warp % 4) * 32 + (i0 + i) * kAtOnce + lane / kChunks, chunk = lane % kChunks;
-                    *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w[i];
+                for (uint32_t i = 0; i < kLoads; ++i) {
+                    w[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row < rows)
+                        w[i] = load_row16<T>(base + (int64_t)tok * a.q_token + (int64_t)head * a.q_head);
+                    row += kAtOnce;
+                    for (head += kAtOnce; head >= a.group; head -= a.group)
+                        ++tok;
                 }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kLoads; ++i) {
+                const uint32_t tr = (warp % 4) * 32 + i * kAtOnce + lane / kChunks;
+                *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w[i];
             }
             fence_proxy_async();
             __syncwarp();
