@@ -191,9 +191,9 @@ BNN_Status encode_map(CUtensorMap* map, const void* base, bool half, uint32_t d,
     return e == CUDA_SUCCESS ? BNN_OK : BNN_EIO;
 }
 
-template <int D, typename T, int kTiles>
+template <int D, typename T, int kMode>
 BNN_Status launch_tiles(BNN_Device device, const AttnArgs& a, cudaStream_t stream, bool every_request) {
-    using Shape = PrefillShape<D, kTiles>;
+    using Shape = PrefillShape<D, kMode>;
     constexpr bool half = std::is_same<T, __half>::value;
     PrefillArgs args;
     args.a = a;
@@ -202,17 +202,18 @@ BNN_Status launch_tiles(BNN_Device device, const AttnArgs& a, cudaStream_t strea
     if (st == BNN_OK)
         st = encode_map(&args.v_map, a.c.v, half, D, a.c, a.c.v_page, a.c.v_head, a.c.v_row);
     if (st == BNN_OK)
-        st = allow_smem(device->ordinal, (const void*)attention_tiles_kernel<D, T, kTiles>, Shape::kSmem);
+        st = allow_smem(device->ordinal, (const void*)attention_tiles_kernel<D, T, kMode>, Shape::kSmem);
     if (st != BNN_OK)
         return st;
-    const uint64_t items = ((uint64_t)a.tokens * a.group) / (kTiles * kPfRows) + a.batch;  // at most
+    const uint64_t items = ((uint64_t)a.tokens * a.group) / (Shape::kQTiles * kPfRows) + a.batch;  // at most
     if (items * a.c.kv_heads > INT32_MAX)
         return BNN_EINVAL;
-    return launch(attention_tiles_kernel<D, T, kTiles>, dim3((uint32_t)(items * a.c.kv_heads)), Shape::kThreads, Shape::kSmem,
+    return launch(attention_tiles_kernel<D, T, kMode>, dim3((uint32_t)(items * a.c.kv_heads)), Shape::kThreads, Shape::kSmem,
                   stream, args);
 }
 
 constexpr uint32_t kMixedCache = 1024;  // positions
+constexpr uint32_t kTurnsCache = 512;
 
 template <int D, typename T>
 BNN_Status attention_typed(BNN_Device device, AttnArgs a, cudaStream_t stream) {
@@ -234,8 +235,14 @@ BNN_Status attention_typed(BNN_Device device, AttnArgs a, cudaStream_t stream) {
             return st;
     }
     const uint64_t pairs = (((uint64_t)a.tokens * a.group) / (2 * kPfRows) + a.batch) * a.c.kv_heads;
-    return pairs >= (uint64_t)device->sm_count ? launch_tiles<D, T, 2>(device, a, stream, !mixed)
-                                               : launch_tiles<D, T, 1>(device, a, stream, !mixed);
+    // Two row tiles in a CTA while such pairs fill the GPU; else one, with two
+    // streams over its keys where there are enough of them (one stream and two:
+    // 256 tokens behind 8192 positions 118 and 93 us, 100 behind 1000 22 and 20 us,
+    // a 512-token prompt 12.7 and 13.2 us, eight of up to 64 tokens 8.0 and 9.2 us).
+    if (pairs >= (uint64_t)device->sm_count)
+        return launch_tiles<D, T, kPair>(device, a, stream, !mixed);
+    return ((uint64_t)a.table_width << a.c.page_shift) > kTurnsCache ? launch_tiles<D, T, kTurns>(device, a, stream, !mixed)
+                                                                     : launch_tiles<D, T, kSingle>(device, a, stream, !mixed);
 }
 
 }  // namespace

@@ -15,7 +15,7 @@ namespace paged {
 // Bits of the handle's paged status word.
 constexpr int kPagedRange = 4;  // position, slot or max_q exceeded; kStatusTimeout: a wait expired
 
-constexpr uint32_t kTypeF32 = 1, kTypeBf16 = 2, kTypeF16 = 3;
+constexpr uint32_t kTypeF32 = 1;  // BNN_PAGED_F32
 
 struct Cache {
     unsigned char* k;

@@ -83,10 +83,11 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Request& r) {
 // This kernel's requests: those whose new tokens and heads fit the 16 rows, and
 // those behind a long cache whose rows make few enough groups of 16 (each group
 // reads the cache again, from L2 mostly). A tile's keys stay on one SM, here
-// they spread over all. 8 KV heads, group 2, tiles against groups: 24 tokens
-// behind 8192 positions 114 and 29 us, 100 tokens 115 and 69 us (104 groups),
-// 200 tokens 117 and 114 us; two requests of 64 behind 4000 60 and 52 us (128
-// groups), four 61 and 83 us; 100 behind 1000 22 and 25 us.
+// they spread over all. 8 KV heads, group 2, pages of 16, tiles against groups:
+// behind 8192 positions 92 us for up to 128 rows against 30 (24 tokens), 69 (100
+// tokens, 104 groups) and 114 us (200 tokens); two requests of 64 behind 4000
+// about the same (128 groups, 52 us), four 57 and 83 us; 100 behind 1000 20 and
+// 25 us.
 __device__ __forceinline__ bool few_rows(const AttnArgs& a, const Request& r) {
     const uint32_t rows = (uint32_t)r.n * a.group;
     return r.n > 0 && (uint32_t)r.n <= a.max_q &&

@@ -11,9 +11,12 @@
 // more than 2^kSlack; then O (TMEM) and l are scaled by 2^(c (m_old - m_new)). The
 // result does not depend on m beyond rounding: weights reach at most 2^kSlack.
 //
-// A CTA holds kTiles tiles of 128 rows that share the K and V tiles: while the
-// tensor core multiplies for one, the other's threads take exponentials.
-// Warps: 4 per tile for the softmax (thread = row = TMEM lane), one that issues
+// A CTA runs one or two such streams; two, so that the tensor core multiplies for one while
+// the other's threads take exponentials: two tiles of 128 rows that share the K
+// and V tiles (kPair), or, where there are too few rows to fill the GPU, one tile
+// of rows whose key tiles the streams take in turn (kTurns), joined at the end as
+// the split kernel joins its parts; short caches are one stream's (kSingle).
+// Warps: 4 per stream for the softmax (thread = row = TMEM lane), one that issues
 // the TMA loads, one that issues the products. K and V arrive page by page
 // (one box of up to 128 rows by 64 columns, 128-byte swizzle) in a ring of
 // 128-key tiles. A position that no row of the CTA sees may hold anything:
@@ -48,20 +51,26 @@ constexpr uint32_t kPfHalf = 64;    // keys whose weights are handed over at onc
 constexpr uint32_t kPfRows = 128;   // rows of a tile
 constexpr float kSlack = 8.0f;      // log2 of the largest weight
 
-template <int D, int kTiles>
+// How a CTA works: one tile of rows; one whose key tiles two streams take in
+// turn; two tiles of rows, a stream each.
+enum Mode { kSingle, kTurns, kPair };
+
+template <int D, int kMode>
 struct PrefillShape {
-    static constexpr uint32_t kThreads = kTiles * 128 + 64;
+    static constexpr uint32_t kStreams = kMode == kSingle ? 1 : 2, kQTiles = kMode == kPair ? 2 : 1;
+    static constexpr uint32_t kThreads = kStreams * 128 + 64;
     static constexpr uint32_t kTileBytes = kPfKeys * D * 2;  // of K, V or Q
-    static constexpr uint32_t kStages = kTiles == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 4 : 8);
+    static constexpr uint32_t kStages = D == 128 ? 5 : 8;
     // 64-wide heads leave TMEM room for P beside S: then Q K^T of the next keys
     // follows as soon as S is in registers, and the softmax need not wait for it
     // (window chunks 198 -> 178 us). 128-wide heads fill the TMEM with S and O, and
     // P takes S's place.
     static constexpr bool kApart = D == 64;
-    static constexpr uint32_t kTmemUsed = kTiles * (kPfKeys + D + (kApart ? kPfHalf : 0));
-    static constexpr uint32_t kTmemCols = kTmemUsed <= 256 ? 256 : 512;
-    static constexpr uint32_t kBars = 2 * kStages + 6 * kTiles + 1;
-    static constexpr size_t kSmem = 1024 + (size_t)(kTiles + kStages) * kTileBytes + kBars * 8 + 16 * 4 + 64;
+    static constexpr uint32_t kTmemCols = kStreams * 256;
+    static_assert(kStreams * (kPfKeys + D + (kApart ? kPfHalf : 0)) <= kTmemCols, "S, O and P of the streams");
+    static constexpr uint32_t kBars = 2 * kStages + 6 * kStreams + kQTiles + 1;
+    static constexpr size_t kSmem = 1024 + (size_t)(kQTiles + kStages) * kTileBytes + kBars * 8 + 16 * 4 + 64;
+    static_assert((D + 2) * kPfRows * 4 <= kStages * kTileBytes, "a stream's O, m and l fit the ring");
 };
 
 struct PrefillArgs {
@@ -171,30 +180,31 @@ __device__ __forceinline__ KeyTiles key_tiles(const AttnArgs& a, int32_t p0, int
     return k;
 }
 
-template <int D, typename T, int kTiles>
-static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
+template <int D, typename T, int kMode>
+static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
     attention_tiles_kernel(const __grid_constant__ PrefillArgs args) {
-    using Shape = PrefillShape<D, kTiles>;
+    using Shape = PrefillShape<D, kMode>;
+    constexpr uint32_t kStreams = Shape::kStreams;
     constexpr uint32_t kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
     constexpr uint32_t kHalves = D / 64;                // 64-column halves of a tile
     constexpr uint32_t kHalfBytes = kPfKeys * 128;      // 16 KB
-    constexpr uint32_t kLoadWarp = kTiles * 4, kMmaWarp = kTiles * 4 + 1;
-    constexpr uint32_t kItemRows = kTiles * kPfRows;
+    constexpr uint32_t kLoadWarp = kStreams * 4, kMmaWarp = kLoadWarp + 1;
+    constexpr uint32_t kQTiles = Shape::kQTiles, kItemRows = kQTiles * kPfRows;
     constexpr bool kApart = Shape::kApart;
     const AttnArgs& a = args.a;
     extern __shared__ __align__(1024) unsigned char pf_smem[];
     const uint32_t raw = smem_addr(pf_smem);
     unsigned char* sm = pf_smem + (((raw + 1023u) & ~1023u) - raw);
     unsigned char* q_sm = sm;
-    unsigned char* ring = sm + kTiles * kTileBytes;
+    unsigned char* ring = sm + kQTiles * kTileBytes;
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + kStages * kTileBytes);
     uint64_t* empty = full + kStages;
-    uint64_t* q_ready = empty + kStages;     // [kTiles] Q in shared memory
-    uint64_t* s_ready = q_ready + kTiles;    // [kTiles] S in TMEM and the last keys' P V done
-    uint64_t* p_ready = s_ready + kTiles;    // [kTiles][2] half of P in TMEM, O scaled
-    uint64_t* s_free = p_ready + 2 * kTiles;  // [kTiles] S in registers (kApart)
-    uint64_t* o_ready = s_free + kTiles;      // [kTiles] P V done (kApart)
-    uint64_t* drained = o_ready + kTiles;
+    uint64_t* q_ready = empty + kStages;   // [kQTiles] Q in shared memory
+    uint64_t* s_ready = q_ready + kQTiles;  // [kStreams] a stream's S in TMEM and its last keys' P V done
+    uint64_t* p_ready = s_ready + kStreams;        // [kStreams][2] half of its P in TMEM, O scaled
+    uint64_t* s_free = p_ready + 2 * kStreams;     // [kStreams] its S in registers (kApart)
+    uint64_t* o_ready = s_free + kStreams;         // [kStreams] its P V done (kApart)
+    uint64_t* drained = o_ready + kStreams;
     uint32_t* mapped = reinterpret_cast<uint32_t*>(drained + 1);  // [16] bit u: 16-key part u of tile t (mod 16) is in memory
     uint32_t* tmem_slot = mapped + 16;
     __shared__ uint32_t warp_sum[32];
@@ -208,8 +218,9 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int t = 0; t < kTiles; ++t) {
-            mbar_init(&q_ready[t], 4);
+        for (uint32_t t = 0; t < kQTiles; ++t)
+            mbar_init(&q_ready[t], kLoadWarp / kQTiles);
+        for (uint32_t t = 0; t < kStreams; ++t) {
             mbar_init(&s_ready[t], 1);
             mbar_init(&p_ready[2 * t], 4);
             mbar_init(&p_ready[2 * t + 1], 4);
@@ -298,26 +309,39 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                                      base_pos + (int32_t)(min(row0 + kItemRows, rows) - 1) / (int32_t)a.group);
     const uint32_t count = tiles.count;
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tmem_o = tmem + kTiles * kPfKeys;
-    const uint32_t tmem_p = kApart ? tmem_o + kTiles * D : tmem, p_step = kApart ? kPfHalf : kPfKeys;  // tile's P
+    const uint32_t tmem_o = tmem + kStreams * kPfKeys;
+    const uint32_t tmem_p = kApart ? tmem_o + kStreams * D : tmem, p_step = kApart ? kPfHalf : kPfKeys;  // a stream's P
 
     if (warp == kLoadWarp) {
         // ---- K and V tiles, page by page: lane p has the tile's p-th page
         const uint32_t page_rows = min(1u << a.c.page_shift, kPfKeys);
         const uint32_t per_tile = kPfKeys / page_rows;
+        constexpr uint32_t kMostPages = kPfKeys / 16;
         uint32_t slot = 0, round = 0;
         const bool starved = *reinterpret_cast<volatile int*>(&g_paged_starve) != 0;
-        for (uint32_t t = 0; t < count; ++t) {
+        // this lane's page of tile t, or -1
+        auto lookup = [&](uint32_t t) -> int32_t {
             const int32_t j = tiles.key(t) + (int32_t)(lane * page_rows);
-            const bool need = lane < per_tile && j <= tiles.last && (j + (int32_t)page_rows > tiles.lo || j < tiles.sink_end);
-            const int32_t page = need ? page_of(a, b, j) : -1;
+            const bool need = t < count && lane < per_tile && j <= tiles.last && (j + (int32_t)page_rows > tiles.lo || j < tiles.sink_end);
+            return need ? page_of(a, b, j) : -1;
+        };
+        int32_t next = lookup(0);
+#pragma unroll 1
+        for (uint32_t t = 0; t < count; ++t) {
+            const int32_t page = next;
+            next = lookup(t + 1);  // on its way while this tile's copies are issued
             const uint32_t parts = page_rows / 16;
             const uint32_t bits =
                 __reduce_or_sync(0xffffffffu, page >= 0 ? ((1u << parts) - 1u) << (lane * parts) : 0u);
             const uint32_t bytes = (uint32_t)__popc(bits) * 16 * D * 2;
-            const int32_t in_page = j & ((1 << a.c.page_shift) - 1);
-            bool ok = true;
+            // only a page longer than a tile is entered at another row than its first
+            const int32_t in_page = tiles.key(t) & ((1 << a.c.page_shift) - 1);
+            int32_t pages[kMostPages];
 #pragma unroll
+            for (uint32_t p = 0; p < kMostPages; ++p)
+                pages[p] = __shfl_sync(0xffffffffu, page, p);
+            bool ok = true;
+#pragma unroll 1
             for (int which = 0; which < 2; ++which) {
                 if (round > 0)
                     ok = wait(&empty[slot], (round - 1) & 1);
@@ -329,12 +353,19 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                     mbar_arrive_expect_tx(&full[slot], bytes);
                 }
                 __syncwarp();
-                if (page >= 0) {
-                    const uint32_t dst = smem_addr(ring + slot * kTileBytes) + lane * page_rows * 128;
+                // one elected thread issues all copies: issued by a lane each, they
+                // took 100 clocks apiece (256 tokens behind 8192 positions in pages of 16:
+                // 119 us that way, 93 us this way; 73 us in pages of 64)
+                if (elect_one()) {
+                    const uint32_t dst = smem_addr(ring + slot * kTileBytes);
+                    const CUtensorMap* map = which ? &args.v_map : &args.k_map;
 #pragma unroll
-                    for (uint32_t h = 0; h < kHalves; ++h)
-                        tma_load_4d(dst + h * kHalfBytes, which ? &args.v_map : &args.k_map, &full[slot], (int32_t)(h * 64),
-                                    in_page, (int32_t)kvh, page);
+                    for (uint32_t p = 0; p < kMostPages; ++p)
+                        if (p < per_tile && pages[p] >= 0)
+#pragma unroll
+                            for (uint32_t h = 0; h < kHalves; ++h)
+                                tma_load_4d(dst + p * page_rows * 128 + h * kHalfBytes, map, &full[slot], (int32_t)(h * 64), in_page,
+                                            (int32_t)kvh, pages[p]);
                 }
                 __syncwarp();
                 if (++slot == kStages) {
@@ -366,61 +397,96 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             };
             auto slot_of = [&](uint32_t t, uint32_t which) { return (2 * t + which) % kStages; };
             auto parity_of = [&](uint32_t t, uint32_t which) { return ((2 * t + which) / kStages) & 1; };
-            auto qk = [&](uint32_t tile, uint32_t t) {
-                const uint64_t qa = q_desc + (tile * kTileBytes >> 4), ka = k_desc + (slot_of(t, 0) * kTileBytes >> 4);
-                const uint32_t to = tmem + tile * kPfKeys;
+            auto qk = [&](uint32_t stream, uint32_t t) {
+                const uint64_t qa = q_desc + ((kMode == kPair ? stream : 0) * kTileBytes >> 4), ka = k_desc + (slot_of(t, 0) * kTileBytes >> 4);
+                const uint32_t to = tmem + stream * kPfKeys;
 #pragma unroll
                 for (uint32_t k = 0; k < D / 16; ++k) {
                     const uint32_t off = ((k / 4) * kHalfBytes + (k % 4) * 32) >> 4;
                     mma_f16_ss(to, qa + off, ka + off, kQkDesc, k != 0);
                 }
             };
-            if (count > 0 && need(&full[slot_of(0, 0)], 0)) {
+            // P V of key tile t, the stream's j-th
+            auto pv = [&](uint32_t stream, uint32_t t, uint32_t j) {
+                const uint64_t va = v_desc + (slot_of(t, 1) * kTileBytes >> 4);
 #pragma unroll 1
-                for (uint32_t tile = 0; tile < kTiles && need(&q_ready[tile], 0); ++tile) {
+                for (uint32_t h = 0; h < 2 && need(&p_ready[2 * stream + h], j & 1); ++h) {
                     tc_fence_after();
-                    qk(tile, 0);
-                    mma_commit(&s_ready[tile]);
+#pragma unroll
+                    for (uint32_t k = 0; k < kPfHalf / 16; ++k)
+                        mma_f16_ts(tmem_o + stream * D, tmem_p + stream * p_step + h * (kPfHalf / 2) + k * 8,
+                                   va + ((h * kPfHalf + k * 16) * 128 >> 4), kPvDesc, j != 0 || h != 0 || k != 0);
+                }
+                return ok;
+            };
+            if (kMode != kTurns && count > 0 && need(&full[slot_of(0, 0)], 0)) {
+#pragma unroll 1
+                for (uint32_t stream = 0; stream < kStreams && need(&q_ready[kMode == kPair ? stream : 0], 0); ++stream) {
+                    tc_fence_after();
+                    qk(stream, 0);
+                    mma_commit(&s_ready[stream]);
                 }
                 mma_commit(&empty[slot_of(0, 0)]);
 #pragma unroll 1
                 for (uint32_t t = 0; ok && t < count; ++t) {
                     const bool more = t + 1 < count;
-                    auto next_scores = [&](uint32_t tile) {
-                        if (more && (tile != 0 || need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0))))
-                            qk(tile, t + 1);
-                        if (more && tile == kTiles - 1)
+                    auto next_scores = [&](uint32_t stream) {
+                        if (more && (stream != 0 || need(&full[slot_of(t + 1, 0)], parity_of(t + 1, 0))))
+                            qk(stream, t + 1);
+                        if (more && stream == kStreams - 1)
                             mma_commit(&empty[slot_of(t + 1, 0)]);
                     };
                     if constexpr (kApart) {
 #pragma unroll 1
-                        for (uint32_t tile = 0; more && tile < kTiles && need(&s_free[tile], t & 1); ++tile) {
+                        for (uint32_t stream = 0; more && stream < kStreams && need(&s_free[stream], t & 1); ++stream) {
                             tc_fence_after();
-                            next_scores(tile);
-                            mma_commit(&s_ready[tile]);
+                            next_scores(stream);
+                            mma_commit(&s_ready[stream]);
                         }
                     }
                     if (!need(&full[slot_of(t, 1)], parity_of(t, 1)))
                         break;
-                    const uint64_t va = v_desc + (slot_of(t, 1) * kTileBytes >> 4);
 #pragma unroll 1
-                    for (uint32_t tile = 0; ok && tile < kTiles; ++tile) {
-#pragma unroll 1
-                        for (uint32_t h = 0; h < 2 && need(&p_ready[2 * tile + h], t & 1); ++h) {
-                            tc_fence_after();
-#pragma unroll
-                            for (uint32_t k = 0; k < kPfHalf / 16; ++k)
-                                mma_f16_ts(tmem_o + tile * D, tmem_p + tile * p_step + h * (kPfHalf / 2) + k * 8,
-                                           va + ((h * kPfHalf + k * 16) * 128 >> 4), kPvDesc, t != 0 || h != 0 || k != 0);
-                        }
-                        if (!ok)
-                            break;
+                    for (uint32_t stream = 0; stream < kStreams && pv(stream, t, t); ++stream) {
                         if constexpr (kApart) {
-                            mma_commit(&o_ready[tile]);
+                            mma_commit(&o_ready[stream]);
                         } else {
-                            next_scores(tile);
-                            mma_commit(&s_ready[tile]);
+                            next_scores(stream);
+                            mma_commit(&s_ready[stream]);
                         }
+                    }
+                    mma_commit(&empty[slot_of(t, 1)]);
+                }
+            }
+            if (kMode == kTurns && count > 0 && need(&q_ready[0], 0)) {
+                // scores of key tile t, and its K tile free again
+                auto scores = [&](uint32_t t) {
+                    if (!need(&full[slot_of(t, 0)], parity_of(t, 0)))
+                        return;
+                    tc_fence_after();
+                    qk(t & 1, t);
+                    mma_commit(&empty[slot_of(t, 0)]);
+                };
+#pragma unroll 1
+                for (uint32_t t = 0; t < min(count, 2u); ++t) {
+                    scores(t);
+                    mma_commit(&s_ready[t]);
+                }
+#pragma unroll 1
+                for (uint32_t t = 0; ok && t < count; ++t) {
+                    const uint32_t stream = t & 1, j = t / 2;
+                    if (kApart && t + 2 < count && need(&s_free[stream], j & 1)) {
+                        scores(t + 2);
+                        mma_commit(&s_ready[stream]);
+                    }
+                    if (!need(&full[slot_of(t, 1)], parity_of(t, 1)) || !pv(stream, t, j))
+                        break;
+                    if (kApart) {
+                        mma_commit(&o_ready[stream]);
+                    } else {
+                        if (t + 2 < count)
+                            scores(t + 2);
+                        mma_commit(&s_ready[stream]);
                     }
                     mma_commit(&empty[slot_of(t, 1)]);
                 }
@@ -435,17 +501,19 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             atomicOr(a.status, kStatusTimeout);
     } else {
         // ---- softmax: thread = row
-        const uint32_t tile = warp / 4, wrow = row0 + tile * kPfRows + (warp % 4) * 32;  // the warp's first row
+        const uint32_t stream = warp / 4, wrow = row0 + (kMode == kPair ? stream * kPfRows : 0) + (warp % 4) * 32;  // the warp's first row
         const uint32_t lane_off = ((warp % 4) * 32u) << 16;
-        const uint32_t t_s = tmem + tile * kPfKeys + lane_off, t_o = tmem_o + tile * D + lane_off;
-        const uint32_t t_p = tmem_p + tile * p_step + lane_off;
+        const uint32_t t_s = tmem + stream * kPfKeys + lane_off, t_o = tmem_o + stream * D + lane_off;
+        const uint32_t t_p = tmem_p + stream * p_step + lane_off;
         {
-            unsigned char* q = q_sm + tile * kTileBytes;
-            constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks;
+            // each warp loads 32 rows of its stream's tile, or 16 of the only one
+            constexpr uint32_t kChunks = D / 8, kAtOnce = 32 / kChunks, kLoadRows = kMode == kTurns ? 16 : 32;
+            unsigned char* q = q_sm + (kMode == kPair ? stream : 0) * kTileBytes;
+            const uint32_t first = kMode == kTurns ? warp * 16 : (warp % 4) * 32;  // in the tile
             const bool q_aligned = ((reinterpret_cast<uintptr_t>(a.q) | (uint64_t)a.q_token * 2 | (uint64_t)a.q_head * 2) & 15u) == 0;
-            constexpr uint32_t kLoads = 32 / kAtOnce;
+            constexpr uint32_t kLoads = kLoadRows / kAtOnce;
             const uint32_t chunk = lane % kChunks;
-            uint32_t row = wrow + lane / kChunks, tok = row / a.group, head = row % a.group;
+            uint32_t row = row0 + (kMode == kPair ? stream * kPfRows : 0) + first + lane / kChunks, tok = row / a.group, head = row % a.group;
             const T* base = reinterpret_cast<const T*>(a.q) + (int64_t)r.start * a.q_token + (int64_t)(kvh * a.group) * a.q_head + chunk * 8;
             uint4 w[kLoads];
             // all of the warp's rows at once, nothing between the loads that would
@@ -473,13 +541,13 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             }
 #pragma unroll
             for (uint32_t i = 0; i < kLoads; ++i) {
-                const uint32_t tr = (warp % 4) * 32 + i * kAtOnce + lane / kChunks;
+                const uint32_t tr = first + i * kAtOnce + lane / kChunks;
                 *reinterpret_cast<uint4*>(q + (chunk / 8) * kHalfBytes + tr * 128 + (((chunk % 8) ^ (tr & 7u)) * 16u)) = w[i];
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0)
-                mbar_arrive(&q_ready[tile]);
+                mbar_arrive(&q_ready[kMode == kPair ? stream : 0]);
         }
         const uint32_t my_row = wrow + lane;
         const int32_t token = (int32_t)min(my_row / a.group, (uint32_t)r.n - 1);
@@ -489,9 +557,11 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
         const float c = a.scale_log2;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
+        const uint32_t steps = kMode == kTurns ? (count + 1 - stream) / 2 : count;  // this stream's
 #pragma unroll 1
-        for (uint32_t t = 0; t < count; ++t) {
-            if (!(ok = wait(&s_ready[tile], t & 1)))
+        for (uint32_t j = 0; j < steps; ++j) {
+            const uint32_t t = kMode == kTurns ? 2 * j + stream : j;  // key tile
+            if (!(ok = wait(&s_ready[stream], j & 1)))
                 break;
             tc_fence_after();
             uint32_t s[kPfKeys];
@@ -500,15 +570,15 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 tmem_ld32(t_s + i * 32, s + i * 32);
             const int32_t key0 = tiles.key(t);
             const uint32_t bits = mapped[t % 16];  // written before the K tile's load, which S came after
-            if (tile == 0 && (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > tiles.last || key0 < tiles.lo)) {
+            if ((kMode == kTurns || stream == 0) && (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > tiles.last || key0 < tiles.lo)) {
                 // V rows that no row of this CTA sees become zeros before the first
-                // product with them (which waits for this tile's P)
+                // product with them (which waits for this stream's P)
                 const uint32_t slot = (2 * t + 1) % kStages;
                 if (!(ok = wait(&full[slot], ((2 * t + 1) / kStages) & 1)))
                     break;
                 unsigned char* v = ring + slot * kTileBytes;
 #pragma unroll 1
-                for (uint32_t row = tid / 8; row < kPfKeys; row += 16) {
+                for (uint32_t row = tid % 128 / 8; row < kPfKeys; row += 16) {
                     const int32_t j = key0 + (int32_t)row;
                     const bool used = (bits >> (row / 16) & 1u) && j <= tiles.last && (j >= tiles.lo || j < tiles.sink_end);
                     if (!used)
@@ -523,7 +593,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive(&s_free[tile]);
+                    mbar_arrive(&s_free[stream]);
             }
             if (bits != 0xffu || key0 + (int32_t)kPfKeys - 1 > first_pos || (a.window && key0 < last_lo)) {
                 // at the edges of what the rows see: hidden scores to -inf
@@ -551,13 +621,13 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
             const bool grow = top > m && (top - m) * c > kSlack;  // also the first finite score
             if constexpr (kApart) {
                 // the last keys' product has read P and is in O
-                if (t > 0 && !(ok = wait(&o_ready[tile], (t - 1) & 1)))
+                if (j > 0 && !(ok = wait(&o_ready[stream], (j - 1) & 1)))
                     break;
                 tc_fence_after();
             }
             if (__any_sync(0xffffffffu, grow)) {
                 const float mn = grow ? top : m, w = grow ? exp2_fast((m - mn) * c) : 1.0f;
-                if (t > 0) {
+                if (j > 0) {
                     // the product of the last keys has completed (s_ready, o_ready)
 #pragma unroll 1
                     for (uint32_t i = 0; i < D / 32; ++i) {
@@ -592,16 +662,49 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0)
-                    mbar_arrive(&p_ready[2 * tile + h]);
+                    mbar_arrive(&p_ready[2 * stream + h]);
             }
             l += (f2_lo(sum2[0]) + f2_hi(sum2[0])) + (f2_lo(sum2[1]) + f2_hi(sum2[1]));
         }
-        if (ok && count > 0)  // every product is in O
-            ok = kApart ? wait(&o_ready[tile], (count - 1) & 1) : wait(&s_ready[tile], count & 1);
+        // every product of stream s is in its O
+        auto finished = [&](uint32_t s, uint32_t n) { return n == 0 || (kApart ? wait(&o_ready[s], (n - 1) & 1) : wait(&s_ready[s], n & 1)); };
+        ok = ok && finished(stream, steps);
+        float* joint = reinterpret_cast<float*>(ring);  // stream 1's O [column][row], then m and l
+        if (kMode == kTurns) {
+            if (stream == 1) {
+                ok = ok && finished(0, (count + 1) / 2);  // then the ring is free
+                tc_fence_after();
+                const uint32_t row = tid % 128;
+                if (ok) {
+#pragma unroll 1
+                    for (uint32_t i = 0; steps > 0 && i < D / 32; ++i) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + i * 32, o);
+                        tmem_wait();
+#pragma unroll
+                        for (uint32_t e = 0; e < 32; ++e)
+                            joint[(i * 32 + e) * kPfRows + row] = __uint_as_float(o[e]);
+                    }
+                    joint[D * kPfRows + row] = m;
+                    joint[(D + 1) * kPfRows + row] = l;
+                }
+            }
+            named_barrier(1, 256);
+        }
         if (!ok && lane == 0)
             atomicOr(a.status, kStatusTimeout);
-        if (ok) {
+        if (ok && (kMode != kTurns || stream == 0)) {
             tc_fence_after();
+            float w0 = 1.0f, w1 = 0.0f;  // of the streams' O
+            if (kMode == kTurns && count > 1) {
+                const uint32_t row = tid % 128;
+                const float m1 = joint[D * kPfRows + row], l1 = joint[(D + 1) * kPfRows + row];
+                const float both = fmaxf(m, m1), from = both == -INFINITY ? 0.0f : both;
+                w0 = exp2_fast((m - from) * c);
+                w1 = exp2_fast((m1 - from) * c);
+                m = both;
+                l = __fmaf_rn(l, w0, l1 * w1);
+            }
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const uint32_t head = kvh * a.group + my_row % a.group;
             const int64_t tok = r.start + (int64_t)(my_row / a.group);
@@ -619,7 +722,10 @@ static __global__ void __launch_bounds__(PrefillShape<D, kTiles>::kThreads, 1)
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    x[e] = l == 0.0f ? 0.0f : __uint_as_float(o[e]) * inv;
+                    float v = __uint_as_float(o[e]);
+                    if (kMode == kTurns && count > 1)
+                        v = __fmaf_rn(joint[(i * 32 + e) * kPfRows + tid % 128], w1, v * w0);
+                    x[e] = l == 0.0f ? 0.0f : v * inv;
                     odd |= !finite32(x[e]);
                 }
                 if (my_row < rows && wide) {
