@@ -24,8 +24,8 @@
 // the product.
 //
 // Bound: the chain S -> softmax -> P -> products -> S of a tile. Of 3850 clocks
-// that a step of 128 keys takes for both row tiles (8192 tokens, 295 us,
-// 0.93 PFLOP/s at the 1.7 GHz that the tensor cores leave) a tile's softmax
+// that a step of 128 keys takes for both row tiles (8192 tokens, 300 us,
+// 0.92 PFLOP/s at the 1.7 GHz that the tensor cores leave) a tile's softmax
 // works 2450 (exponentials 1420: 128 a row at 16 a clock and SM are 1024) and
 // waits 1400 for products and hand-overs; MUFU and tensor pipe are each busy
 // half of the time. The TMEM holds S and O of two tiles of 128-wide heads and no
