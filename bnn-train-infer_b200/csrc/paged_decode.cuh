@@ -379,9 +379,11 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
 
     // a row that came out infinite or NaN may owe it to a value that only later
     // tokens see: again, key by key (one token: every key counts)
+    // (`first_bit`: where this row's 16 bits of odd_rows begin; two cut rows are
+    // noted before either is computed again)
     auto redo = [&](const Segment& s, uint32_t first_bit) {
         __syncthreads();
-        if (const uint32_t odd = odd_rows >> first_bit) {
+        if (const uint32_t odd = odd_rows >> first_bit & 0xffffu) {
             if (s.r.n > 1)
 #pragma unroll 1
                 for (uint32_t row = warp; row < kDecRows; row += kDecWarps)
@@ -389,7 +391,7 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                         attention_row<D, T>(a, s.b, s.r, (int32_t)((s.first + row) / a.group), s.kvh * a.group + (s.first + row) % a.group);
             __syncthreads();
             if (tid == 0)
-                odd_rows &= (1u << first_bit) - 1u;
+                odd_rows &= ~(0xffffu << first_bit);
             __syncthreads();
         }
     };
