@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -278,6 +279,90 @@ PyObject* stream(PyObject*, PyObject* device) {
     });
 }
 
+// Who used a workspace last: the stream of the last call outside captures, and
+// the last captured call's with its capture. Calls of unlike captures, and a
+// captured call and one outside, are ordered by whoever replays the graph.
+struct Order {
+    cudaStream_t last;
+    cudaStream_t captured;
+    unsigned long long capture;  // 0: none yet
+    cudaEvent_t event;
+};
+
+void drop_order(PyObject* capsule) {
+    if (Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, "bnn_b200.paged.order"))) {
+        cudaEventDestroy(u->event);
+        delete u;
+    }
+}
+
+void cuda_ok(cudaError_t e, const char* what) {
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        refuse(BNN_EIO, "%s: %s", what, cudaGetErrorString(e));
+    }
+}
+
+// The capture that `stream` is part of, 0 where it is in none.
+unsigned long long capture_of(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream beside somebody's capture
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+void after(cudaStream_t now, cudaStream_t before, cudaEvent_t event) {
+    cuda_ok(cudaEventRecord(event, before), "workspace order");
+    cuda_ok(cudaStreamWaitEvent(now, event, 0), "workspace order");
+}
+
+// new_order(device) -> a workspace's order; its memory is of the current stream
+PyObject* new_order(PyObject*, PyObject* device) {
+    return guarded([&]() -> PyObject* {
+        const auto d = (c10::DeviceIndex)integer(device, "device");
+        const c10::cuda::CUDAGuard guard(d);
+        cudaEvent_t event;
+        cuda_ok(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "workspace order");
+        PyObject* capsule = PyCapsule_New(new Order{c10::cuda::getCurrentCUDAStream(d).stream(), nullptr, 0, event},
+                                          "bnn_b200.paged.order", drop_order);
+        return capsule;
+    });
+}
+
+// order(order, device): the current stream's next work runs after the work that
+// used the workspace before
+PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 2)
+            refuse(BNN_EINVAL, "order: 2 arguments");
+        Order* u = static_cast<Order*>(PyCapsule_GetPointer(o[0], "bnn_b200.paged.order"));
+        if (!u)
+            return nullptr;
+        const auto d = (c10::DeviceIndex)integer(o[1], "device");
+        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
+        if (const unsigned long long capture = capture_of(now)) {
+            // branches of one graph: an edge from the earlier to the later
+            if (u->capture == capture && u->captured != now) {
+                const c10::cuda::CUDAGuard guard(d);
+                after(now, u->captured, u->event);
+            }
+            u->capture = capture;
+            u->captured = now;
+        } else if (u->last != now) {
+            // waiting for a stream that is being captured would draw this one in
+            if (capture_of(u->last) != 0)
+                refuse(BNN_EBUSY, "the stream of the last call is being captured");
+            const c10::cuda::CUDAGuard guard(d);
+            after(now, u->last, u->event);
+            u->last = now;
+        }
+        Py_RETURN_NONE;
+    });
+}
+
 // bind(address of bnn_b200_paged_append, of bnn_b200_paged_attention, BnnError)
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *f, *g, *error;
@@ -295,6 +380,8 @@ PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"stream", stream, METH_O, nullptr},
+    {"new_order", new_order, METH_O, nullptr},
+    {"order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(order)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -45,10 +45,13 @@ def _bind():
 class Paged:
     """The paged-cache operators of one device handle (accel.Device), with their workspace.
 
-    Calls on one stream run in order and share the workspace; a call on
-    another stream first waits for the work the previous one had enqueued.
-    A CUDA graph that captured a call uses the workspace too: replay it in
-    order with the other calls. max_batch: most requests of a call, a bound of
+    Calls on one stream run in order and share the workspace; an attention call
+    on another stream first waits for the work that the stream of the previous
+    one holds, so that stream has to exist still (BNN_EBUSY where it is being
+    captured by then). Captured calls on branches of one CUDA graph are ordered
+    likewise. The graph uses the workspace when it is replayed: replay it in
+    order with the other calls, and keep this object as long as the graph.
+    max_batch: most requests of a call, a bound of
     the program's own (calls beyond it are refused; the library's is 4096)."""
 
     def __init__(self, device: accel.Device, max_batch=4096):
@@ -62,15 +65,7 @@ class Paged:
         if st != OK:
             raise BnnError(st, "bnn_b200_paged_workspace")
         self._workspace = torch.zeros(need.value, dtype=torch.uint8, device=f"cuda:{self._index}")
-        self._stream = torch.cuda.current_stream(self._index)
-        self._raw_stream = self._stream.cuda_stream
-
-    def _other_stream(self, raw):
-        """Orders the workspace's earlier work before the current stream's."""
-        if not torch.cuda.is_current_stream_capturing():
-            now = torch.cuda.current_stream(self._index)
-            now.wait_stream(self._stream)
-            self._stream, self._raw_stream = now, raw
+        self._order = _paged_torch.new_order(self._index)
 
     def append(self, q, k, v, cos, sin, positions, slots, k_pages, v_pages, *, q_norm=None, k_norm=None, eps=1e-6, interleaved=False,
                out=None):
@@ -92,9 +87,7 @@ class Paged:
                 raise BnnError(EINVAL, "out_dtype: q's type or float32, and out's")
         if page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
-        raw = _paged_torch.stream(self._index)
-        if raw != self._raw_stream:
-            self._other_stream(raw)
+        _paged_torch.order(self._order, self._index)
         return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q,
                                       scale, window, sinks, out, f32, return_lse)
 

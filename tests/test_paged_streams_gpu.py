@@ -1,0 +1,127 @@
+"""The workspace of the paged attention between streams and graph branches
+(marked gpu)."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_paged_gpu import BF16, make, ops  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+KERNEL_NODE = 0
+
+
+def captured_edges(graph):
+    """(kernel nodes, edges) of a captured graph."""
+    rt = ctypes.CDLL("libcudart.so.12")
+    raw = ctypes.c_void_p(graph.raw_cuda_graph())
+    count = ctypes.c_size_t()
+    assert rt.cudaGraphGetNodes(raw, None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert rt.cudaGraphGetNodes(raw, nodes, ctypes.byref(count)) == 0
+    kernels = []
+    for node in nodes:
+        kind = ctypes.c_int()
+        assert rt.cudaGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == KERNEL_NODE:
+            kernels.append(node)
+    assert rt.cudaGraphGetEdges_v2(raw, None, None, None, ctypes.byref(count)) == 0
+    if count.value == 0:
+        return kernels, set()
+    first, second = (ctypes.c_void_p * count.value)(), (ctypes.c_void_p * count.value)()
+    data = (ctypes.c_uint64 * count.value)()  # eight bytes an edge
+    assert rt.cudaGraphGetEdges_v2(raw, first, second, data, ctypes.byref(count)) == 0
+    return kernels, set(zip(first, second))
+
+
+def fork(ops, calls):  # noqa: F811
+    """A graph with each call on a branch of its own."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    sides = [torch.cuda.Stream() for _ in calls[1:]]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        for side in sides:
+            side.wait_stream(main)
+        for stream, (made, max_q, out) in zip([main] + sides, calls):
+            with torch.cuda.stream(stream):
+                ops.attention(*made, max_q=max_q, out=out)
+        for side in sides:
+            main.wait_stream(side)
+    return graph
+
+
+def some_calls():
+    calls = []
+    for seed, requests in enumerate(([(1, 9000), (1, 500)], [(2, 5000), (1, 7000), (1, 12)], [(1, 3000)] * 5)):
+        made = make(requests, 8, 2, 128, 64, BF16, seed=seed)
+        calls.append((made, max(n for n, _ in requests), torch.empty_like(made[0])))
+    return calls
+
+
+def test_branches_of_a_graph_are_ordered(ops):  # noqa: F811
+    for _ in range(2):  # also in a second capture
+        graph = fork(ops, some_calls())
+        kernels, edges = captured_edges(graph)
+        assert len(kernels) == 3
+        reach = {k: {b for a, b in edges if a == k} for k in kernels}
+        for _ in kernels:
+            reach = {k: r.union(*(reach[x] for x in r)) for k, r in reach.items()}
+        assert sorted(len(r) for r in reach.values()) == [0, 1, 2]
+        del graph
+
+
+def test_replayed_branches_agree(ops):  # noqa: F811
+    calls = some_calls()
+    want = [ops.attention(*made, max_q=max_q) for made, max_q, _ in calls]
+    graph = fork(ops, calls)
+    for _ in range(20):
+        for _, _, out in calls:
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, out), w in zip(calls, want):
+            assert torch.equal(out, w)
+    again = [ops.attention(*made, max_q=max_q) for made, max_q, _ in calls]
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    ops.sync()
+    del graph
+
+
+def test_a_stream_under_capture_is_not_waited_for(ops):  # noqa: F811
+    """A call outside a capture, with the previous one's stream inside: refused, and neither is drawn into the other."""
+    from bnn_b200 import accel
+    made, max_q, out = some_calls()[0]
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = ops.attention(*made, max_q=max_q)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        ops.attention(*made, max_q=max_q, out=out)
+        with torch.cuda.stream(other), pytest.raises(accel.BnnError) as e:
+            ops.attention(*made, max_q=max_q, out=torch.empty(0))
+        assert e.value.status == accel.EBUSY
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert torch.equal(ops.attention(*made, max_q=max_q), want)
+    del graph
+
+
+@pytest.mark.parametrize("rounds", [30])
+def test_calls_on_many_streams(ops, rounds):  # noqa: F811
+    calls = some_calls()
+    want = [ops.attention(*made, max_q=max_q) for made, max_q, _ in calls]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(rounds):
+        with torch.cuda.stream(streams[i * 7 % 4]):
+            made, max_q, _ = calls[i % 3]
+            got.append(ops.attention(*made, max_q=max_q))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 3])
