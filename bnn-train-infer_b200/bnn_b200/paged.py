@@ -17,6 +17,7 @@ tensors are read and checked in binding/paged_torch.cpp, built beside this
 file by the package Makefile; without it the import raises.
 """
 import ctypes
+import threading
 
 import torch
 
@@ -49,7 +50,7 @@ class Paged:
     on another stream first waits for the work that the stream of the previous
     one holds, so that stream has to exist still (BNN_EBUSY where it is being
     captured by then). Captured calls on branches of one CUDA graph are ordered
-    likewise. The graph uses the workspace when it is replayed: replay it in
+    likewise, and threads may share the object. The graph uses the workspace when it is replayed: replay it in
     order with the other calls, and keep this object as long as the graph.
     max_batch: most requests of a call, a bound of
     the program's own (calls beyond it are refused; the library's is 4096)."""
@@ -66,6 +67,7 @@ class Paged:
             raise BnnError(st, "bnn_b200_paged_workspace")
         self._workspace = torch.zeros(need.value, dtype=torch.uint8, device=f"cuda:{self._index}")
         self._order = _paged_torch.new_order(self._index)
+        self._turn = threading.Lock()
 
     def append(self, q, k, v, cos, sin, positions, slots, k_pages, v_pages, *, q_norm=None, k_norm=None, eps=1e-6, interleaved=False,
                out=None):
@@ -87,9 +89,10 @@ class Paged:
                 raise BnnError(EINVAL, "out_dtype: q's type or float32, and out's")
         if page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
-        _paged_torch.order(self._order, self._index)
-        return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q,
-                                      scale, window, sinks, out, f32, return_lse)
+        with self._turn:  # another thread's call comes before both or after both
+            _paged_torch.order(self._order, self._index)
+            return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts,
+                                          max_q, scale, window, sinks, out, f32, return_lse)
 
     def sync(self):
         """Waits for the current stream; raises what the calls since the last sync recorded

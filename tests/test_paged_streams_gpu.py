@@ -125,3 +125,34 @@ def test_calls_on_many_streams(ops, rounds):  # noqa: F811
     torch.cuda.synchronize()
     for i, x in enumerate(got):
         assert torch.equal(x, want[i % 3])
+
+
+def test_threads_share_a_workspace(ops):  # noqa: F811
+    """Four threads, each on a stream of its own, call at once; every result is the lone call's."""
+    import sys
+    import threading
+    calls = some_calls()
+    want = [ops.attention(*made, max_q=max_q) for made, max_q, _ in calls]
+    torch.cuda.synchronize()
+    wrong, begin = [], threading.Barrier(4)
+
+    def work(nth):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            begin.wait()
+            for i in range(100):
+                made, max_q, _ = calls[(i + nth) % 3]
+                if not torch.equal(ops.attention(*made, max_q=max_q), want[(i + nth) % 3]):
+                    wrong.append((nth, i))
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert not wrong
+    ops.sync()
