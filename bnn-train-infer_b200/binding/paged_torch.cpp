@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -332,17 +333,20 @@ PyObject* new_order(PyObject*, PyObject* device) {
     });
 }
 
-// order(order, device): the current stream's next work runs after the work that
-// used the workspace before
+// order(order, device, workspace): the current stream's next work runs after the
+// work that used the workspace before; the memory, which belongs to the stream
+// it was allocated on, is not handed out again before this stream is done with it
 PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 2)
-            refuse(BNN_EINVAL, "order: 2 arguments");
+        if (n != 3)
+            refuse(BNN_EINVAL, "order: 3 arguments");
         Order* u = static_cast<Order*>(PyCapsule_GetPointer(o[0], "bnn_b200.paged.order"));
         if (!u)
             return nullptr;
         const auto d = (c10::DeviceIndex)integer(o[1], "device");
-        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
+        const at::Tensor& workspace = tensor(o[2], "workspace");
+        const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(d);
+        const cudaStream_t now = current.stream();
         if (const unsigned long long capture = capture_of(now)) {
             // branches of one graph: an edge from the earlier to the later
             if (u->capture == capture && u->captured != now) {
@@ -357,6 +361,7 @@ PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
                 refuse(BNN_EBUSY, "the stream of the last call is being captured");
             const c10::cuda::CUDAGuard guard(d);
             after(now, u->last, u->event);
+            c10::cuda::CUDACachingAllocator::recordStream(workspace.storage().data_ptr(), current);
             u->last = now;
         }
         Py_RETURN_NONE;

@@ -90,7 +90,7 @@ class Paged:
         if page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
         with self._turn:  # another thread's call comes before both or after both
-            _paged_torch.order(self._order, self._index)
+            _paged_torch.order(self._order, self._index, self._workspace)
             return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts,
                                           max_q, scale, window, sinks, out, f32, return_lse)
 

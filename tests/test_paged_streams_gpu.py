@@ -156,3 +156,24 @@ def test_threads_share_a_workspace(ops):  # noqa: F811
         sys.setswitchinterval(interval)
     assert not wrong
     ops.sync()
+
+
+def test_a_dropped_workspace_waits_for_other_streams(ops):  # noqa: F811
+    """An operators' object that goes while another stream works on its workspace: the memory is not handed out."""
+    from bnn_b200 import paged
+    made, max_q, _ = some_calls()[0]
+    want = ops.attention(*made, max_q=max_q)
+    torch.cuda.synchronize()
+    own = paged.Paged(ops.device)
+    size, at = own._workspace.numel(), own._workspace.data_ptr()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        own.attention(*made, max_q=max_q)
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        got = own.attention(*made, max_q=max_q)
+    del own
+    fresh = torch.empty(size, dtype=torch.uint8, device="cuda")
+    assert not side.query()
+    assert fresh.data_ptr() != at
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
