@@ -58,6 +58,7 @@ class Paged:
     def __init__(self, device: accel.Device, max_batch=4096):
         self._dll = _bind()
         self.device = device
+        self._check_open()
         self._handle = device.handle.value
         self._index = self._dll.bnn_b200_device_ordinal(device.handle)
         self._max_batch = max_batch
@@ -69,10 +70,15 @@ class Paged:
         self._order = _paged_torch.new_order(self._index)
         self._turn = threading.Lock()
 
+    def _check_open(self):
+        if not self.device.handle:
+            raise BnnError(EINVAL, "the device is closed")
+
     def append(self, q, k, v, cos, sin, positions, slots, k_pages, v_pages, *, q_norm=None, k_norm=None, eps=1e-6, interleaved=False,
                out=None):
         """Normalises and rotates q and k, writes k and v to their slots; returns q
         (bnn_b200_paged_append). cos and sin None: no rotation."""
+        self._check_open()
         return _paged_torch.append(self._handle, self._index, q, k, v, cos, sin, positions, slots, k_pages, v_pages, q_norm, k_norm, eps,
                                    interleaved, out)
 
@@ -82,6 +88,7 @@ class Paged:
         (bnn_b200_paged_attention); scale None: 1 / sqrt(head_dim). Returns
         [tokens, heads, head_dim] of q's type (or out_dtype float32), and with
         return_lse the float32 logarithms of the softmax sums [tokens, heads]."""
+        self._check_open()
         f32 = False
         if out_dtype is not None:
             f32 = out_dtype == torch.float32

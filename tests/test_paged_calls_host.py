@@ -8,7 +8,7 @@ import types
 import pytest
 
 torch = pytest.importorskip("torch")
-from bnn_b200 import paged  # noqa: E402
+from bnn_b200 import accel, paged  # noqa: E402
 
 
 class Recorder:
@@ -62,3 +62,14 @@ def test_order_and_launch_are_one_step_between_threads(recorded):
     assert len(recorder.seen) == 160
     for first, second in zip(recorder.seen[::2], recorder.seen[1::2]):
         assert first[0] == second[0] and (first[1], second[1]) == ("order", "attention")
+
+
+def test_a_closed_device_is_refused(recorded):
+    """The handle is gone: nothing that was kept of it reaches the library."""
+    ops, recorder = recorded
+    ops.device.handle = None
+    for call in (lambda: ops.append(*[None] * 9), lambda: ops.attention(*ARGS, max_q=1), lambda: paged.Paged(ops.device)):
+        with pytest.raises(accel.BnnError) as e:
+            call()
+        assert e.value.status == accel.EINVAL
+    assert not recorder.seen
