@@ -13,7 +13,7 @@ namespace bnn {
 namespace paged {
 
 // Bits of the handle's paged status word.
-constexpr int kPagedRange = 4;  // position, slot or max_q exceeded; kStatusTimeout: a wait expired
+constexpr int kPagedRange = 4;  // a position, slot, length, offset or max_q exceeded; kStatusTimeout: a wait expired
 
 constexpr uint32_t kTypeF32 = 1;  // BNN_PAGED_F32
 
@@ -99,19 +99,18 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
 __device__ __forceinline__ bool finite32(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // One request of the call: n new tokens, the first of them token `start` of
-// the batch, behind a cache of kv positions. Malformed offsets and lengths are
-// brought into the tensors' bounds.
+// the batch, behind a cache of kv positions.
 struct Request {
     int32_t start, n, kv;
 };
 
-__device__ __forceinline__ Request load_request(const AttnArgs& a, uint32_t b) {
-    Request r;
-    const int32_t tokens = (int32_t)a.tokens;
-    r.start = min(max(a.q_starts[b], 0), tokens);
-    r.n = max(min(a.q_starts[b + 1], tokens) - r.start, 0);
-    r.kv = min(max(a.kv_lens[b], 0), (int32_t)min((uint64_t)a.table_width << a.c.page_shift, (uint64_t)1 << 30));
-    return r;
+// *bad: the request has tokens outside the call's, or a length that is negative
+// or more than its page table holds; it is left out (n = 0) and reported.
+__device__ __forceinline__ Request load_request(const AttnArgs& a, uint32_t b, bool* bad) {
+    const int32_t begin = a.q_starts[b], end = a.q_starts[b + 1], kv = a.kv_lens[b];
+    const int32_t room = (int32_t)min((uint64_t)a.table_width << a.c.page_shift, (uint64_t)1 << 30);
+    *bad = end > begin && (begin < 0 || end > (int32_t)a.tokens || kv < 0 || kv > room);
+    return Request{begin, end > begin && !*bad ? end - begin : 0, min(max(kv, 0), room)};
 }
 
 // First position of the window of a token at position p (0 without a window).

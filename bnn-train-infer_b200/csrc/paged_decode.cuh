@@ -227,9 +227,10 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
         const uint32_t b = b0 + tid;
         uint32_t x = 0;
         if (b < a.batch) {
-            const Request r = load_request(a, b);
+            bool bad;
+            const Request r = load_request(a, b, &bad);
             requests[b] = r;
-            if (r.n > (int32_t)a.max_q && blockIdx.x == 0)
+            if ((bad || r.n > (int32_t)a.max_q) && blockIdx.x == 0)
                 atomicOr(a.status, kPagedRange);
             x = few_rows(a, r) ? (span_of(a, r).count + kRowCost) * a.c.kv_heads * row_groups(a, r) : 0;
         }

@@ -240,8 +240,9 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
     auto scan = [&](uint32_t b, uint32_t seen) {
         x = 0;
         if (b < a.batch) {
-            mine = load_request(a, b);
-            if (mine.n > (int32_t)a.max_q) {
+            bool bad;
+            mine = load_request(a, b, &bad);
+            if (bad || mine.n > (int32_t)a.max_q) {
                 if (blockIdx.x == 0)
                     atomicOr(a.status, kPagedRange);
             } else if (mine.n > 0 && (args.every_request || !few_rows(a, mine))) {

@@ -23,8 +23,9 @@
  * waiting; they can be captured into a CUDA graph. All pointers are device
  * pointers on the handle's GPU. Strides and sizes count elements. What only
  * the device sees (a position outside the rotation table, a slot outside the
- * cache, a request with more new tokens than max_q) is recorded and read by
- * bnn_b200_paged_sync.
+ * cache, a request with more new tokens than max_q, with tokens outside the
+ * call's or with a length that its page table does not hold) is recorded and
+ * read by bnn_b200_paged_sync.
  */
 #ifndef BNN_B200_PAGED_H
 #define BNN_B200_PAGED_H
@@ -101,9 +102,10 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
  * cache's type (as any 16-bit tensor-core product), the result is rounded once
  * to out_type. lse (natural log of the softmax sum) may be NULL.
  * q has the cache's type; heads is a multiple of kv_heads, at most
- * BNN_PAGED_MAX_GROUP times. max_q bounds the new tokens of any request; the
- * tokens of a request that has more stay unwritten and the next
- * bnn_b200_paged_sync returns BNN_ERANGE. workspace: bnn_b200_paged_workspace
+ * BNN_PAGED_MAX_GROUP times. max_q bounds the new tokens of any request. The
+ * tokens of a request that has more of them, or some outside [0, tokens), or a
+ * kv_len below zero or above table_width * page_size, stay unwritten and the
+ * next bnn_b200_paged_sync returns BNN_ERANGE. workspace: bnn_b200_paged_workspace
  * bytes, zeroed once before its first use and used by one call at a time
  * (calls on one stream may share it). Results do not depend on what else is
  * in flight: sums are joined in a fixed order. */
