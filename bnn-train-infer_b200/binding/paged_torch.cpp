@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -79,6 +80,15 @@ void on_device(const at::Tensor& x, int device, const char* name) {
         refuse(BNN_EINVAL, "%s: not on cuda:%d", name, device);
 }
 
+// These operators have no derivative: a tensor that wants one, of either mode, is
+// refused wherever it would be dropped.
+void no_gradient(const at::Tensor& x, const char* name) {
+    if (x.requires_grad() && c10::GradMode::is_enabled())
+        refuse(BNN_EINVAL, "%s requires a gradient, and the paged operators have no backward pass", name);
+    if (x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        refuse(BNN_EINVAL, "%s has a tangent, and the paged operators have no forward-mode derivative", name);
+}
+
 void set_cache(const at::Tensor& k, const at::Tensor& v, int device, BNN_PagedCache* c) {
     if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
         refuse(BNN_EINVAL, "k_pages and v_pages: one shape [pages, kv_heads, page_size, head_dim] and type");
@@ -87,6 +97,8 @@ void set_cache(const at::Tensor& k, const at::Tensor& v, int device, BNN_PagedCa
         refuse(BNN_EINVAL, "k_pages: bfloat16 or float16");
     on_device(k, device, "k_pages");
     on_device(v, device, "v_pages");
+    no_gradient(k, "k_pages");
+    no_gradient(v, "v_pages");
     c->pages = k.size(0);
     c->kv_heads = k.size(1);
     c->page_size = k.size(2);
@@ -122,12 +134,8 @@ const E* vector(PyObject* o, const char* name, at::ScalarType type, int64_t coun
     if (x.scalar_type() != type || x.dim() != 1 || x.size(0) != count || (count > 1 && x.stride(0) != 1))
         refuse(BNN_EINVAL, "%s: %lld adjacent %s are wanted", name, (long long)count, at::toString(type));
     on_device(x, device, name);
+    no_gradient(x, name);
     return static_cast<const E*>(x.data_ptr());
-}
-
-void no_backward(const at::Tensor& x, const char* what) {
-    if (x.requires_grad() && c10::GradMode::is_enabled())
-        refuse(BNN_EINVAL, "%s has no backward pass", what);
 }
 
 at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, int device) {
@@ -163,9 +171,9 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         d.type = type_of(q.scalar_type());
         if (d.type == 0 || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
             refuse(BNN_EINVAL, "q, k and v: one type, float32, bfloat16 or float16");
-        no_backward(q, "append");
-        no_backward(k, "append");
-        no_backward(v, "append");
+        no_gradient(q, "q");
+        no_gradient(k, "k");
+        no_gradient(v, "v");
         const int64_t dim = d.cache.head_dim;
         rows(q, "q", d.tokens, d.heads, dim, device, &d.q_token_stride, &d.q_head_stride);
         rows(k, "k", d.tokens, d.cache.kv_heads, dim, device, &d.k_token_stride, &d.k_head_stride);
@@ -180,6 +188,8 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
                 refuse(BNN_EINVAL, "cos and sin: contiguous float32 [positions, rotary_dim / 2]");
             on_device(cos, device, "cos");
             on_device(sin, device, "sin");
+            no_gradient(cos, "cos");
+            no_gradient(sin, "sin");
             d.cos = static_cast<const float*>(cos.data_ptr());
             d.sin = static_cast<const float*>(sin.data_ptr());
             d.table_rows = cos.size(0);
@@ -198,6 +208,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
             out = tensor(o[15], "out");
             if (out.scalar_type() != k_pages.scalar_type())
                 refuse(BNN_EINVAL, "out: the cache's type");
+            no_gradient(out, "out");
         }
         rows(out, "out", d.tokens, d.heads, dim, device, &d.out_token_stride, &d.out_head_stride);
         d.q_out = out.data_ptr();
@@ -223,7 +234,7 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const int64_t dim = d.cache.head_dim;
         if (q.dim() != 3 || q.scalar_type() != k_pages.scalar_type())
             refuse(BNN_EINVAL, "q: [tokens, heads, head_dim] of the cache's type");
-        no_backward(q, "attention");
+        no_gradient(q, "q");
         d.tokens = q.size(0);
         d.heads = q.size(1);
         rows(q, "q", d.tokens, d.heads, dim, device, &d.q_token_stride, &d.q_head_stride);
@@ -247,6 +258,7 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
             out = empty({d.tokens, d.heads, dim}, PyObject_IsTrue(o[14]) == 1 ? at::kFloat : q.scalar_type(), device);
         } else {
             out = tensor(o[13], "out");
+            no_gradient(out, "out");
         }
         rows(out, "out", d.tokens, d.heads, dim, device, &d.out_token_stride, &d.out_head_stride);
         d.out = out.data_ptr();

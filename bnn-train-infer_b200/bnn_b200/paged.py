@@ -12,8 +12,9 @@ runs on torch's current stream and returns without waiting. Shapes:
   cos, sin          [positions, rotary_dim / 2] float32
 
 Like the other wrappers it raises accel.BnnError carrying the status. The
-operators have no backward pass (the library serves trained weights). The
-tensors are read and checked in binding/paged_torch.cpp, built beside this
+operators have no derivatives (the library serves trained weights): a tensor
+that requires a gradient, trained gains among them, is refused outside
+torch.no_grad(). The tensors are read and checked in binding/paged_torch.cpp, built beside this
 file by the package Makefile; without it the import raises.
 """
 import ctypes
