@@ -128,6 +128,13 @@ void rows(const at::Tensor& x, const char* name, int64_t tokens, int64_t heads, 
     *head_stride = x.stride(1);
 }
 
+// A call has been launched that writes x: what autograd saved of it is stale
+// (inference tensors keep no count).
+void written(const at::Tensor& x) {
+    if (!x.is_inference())
+        x.unsafeGetTensorImpl()->bump_version();
+}
+
 template <typename E>
 const E* vector(PyObject* o, const char* name, at::ScalarType type, int64_t count, int device) {
     const at::Tensor& x = tensor(o, name);
@@ -162,8 +169,8 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         const int device = (int)integer(o[1], "device");
         BNN_PagedAppend d = {};
         const at::Tensor &q = tensor(o[2], "q"), &k = tensor(o[3], "k"), &v = tensor(o[4], "v");
-        const at::Tensor& k_pages = tensor(o[9], "k_pages");
-        set_cache(k_pages, tensor(o[10], "v_pages"), device, &d.cache);
+        const at::Tensor &k_pages = tensor(o[9], "k_pages"), &v_pages = tensor(o[10], "v_pages");
+        set_cache(k_pages, v_pages, device, &d.cache);
         if (q.dim() != 3)
             refuse(BNN_EINVAL, "q: [tokens, heads, head_dim]");
         d.tokens = q.size(0);
@@ -216,6 +223,10 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
                                        c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream());
         if (st != BNN_OK)
             refuse(st, "bnn_b200_paged_append");
+        written(k_pages);
+        written(v_pages);
+        if (o[15] != Py_None)
+            written(out);
         return THPVariable_Wrap(out);
     });
 }
@@ -275,6 +286,8 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
                                           c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream());
         if (st != BNN_OK)
             refuse(st, "bnn_b200_paged_attention");
+        if (o[13] != Py_None)
+            written(out);
         if (!want_lse)
             return THPVariable_Wrap(out);
         PyObject *a = THPVariable_Wrap(out), *b = a ? THPVariable_Wrap(lse) : nullptr;

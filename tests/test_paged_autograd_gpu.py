@@ -59,3 +59,31 @@ def test_tangents_are_refused(ops, operator, name):  # noqa: F811
         assert e.value.status == accel.EINVAL
     call(**tensors, **extra)
     ops.sync()
+
+
+@pytest.mark.parametrize("operator,names", [("append", ("k_pages", "v_pages", "out")), ("attention", ("out",))])
+def test_writes_are_counted(ops, operator, names):  # noqa: F811
+    """A tensor that autograd saved and an operator then wrote: backward refuses it, as after any in-place operation."""
+    tensors = append_tensors() if operator == "append" else attention_tensors()
+    extra = {} if operator == "append" else {"max_q": 1}
+    counts = {n: t._version for n, t in tensors.items()}
+    losses = []
+    for n in names:
+        w = torch.ones((), device="cuda", dtype=tensors[n].dtype, requires_grad=True)
+        losses.append((tensors[n] * w).sum())  # saves tensors[n]
+    getattr(ops, operator)(**tensors, **extra)
+    ops.sync()
+    assert {n for n, t in tensors.items() if t._version != counts[n]} == set(names)
+    for loss in losses:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_inference_tensors_are_taken(ops):  # noqa: F811
+    with torch.inference_mode():
+        a, b = append_tensors(), attention_tensors()
+        ops.append(**a)
+        ops.attention(**b, max_q=1)
+    ops.append(**a)
+    ops.attention(**b, max_q=1)
+    ops.sync()
