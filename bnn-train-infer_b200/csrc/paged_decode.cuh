@@ -173,7 +173,8 @@ struct Segment {
 };
 
 // Scales and writes four values of one output row (and its lse with d == 0);
-// notes a row that is not finite.
+// notes a row that is not finite although its sum is a number (a score that is
+// none is one that the row sees).
 template <typename T>
 __device__ __noinline__ void finish4(const AttnArgs& a, const Segment& s, uint32_t in_group, uint32_t d, float4 p, float sum, float mm,
                                      uint32_t* odd_rows, uint32_t bit) {
@@ -183,7 +184,7 @@ __device__ __noinline__ void finish4(const AttnArgs& a, const Segment& s, uint32
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         v[e] = sum == 0.0f ? 0.0f : v[e];
-        if (!finite32(v[e]))
+        if (!finite32(v[e]) && !isnan(sum))
             atomicOr(odd_rows, 1u << bit);
     }
     store_out4<T>(a, (int64_t)tok * a.o_token + (int64_t)head * a.o_head + d, v);
@@ -378,18 +379,18 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
     for (uint32_t s = 0; s < kStages - 1; ++s)
         fetch();
 
-    // a row that came out infinite or NaN may owe it to a value that only later
-    // tokens see: again, key by key (one token: every key counts)
+    // a row that came out infinite or NaN may owe it to a value that only other
+    // tokens see (attention_row)
     // (`first_bit`: where this row's 16 bits of odd_rows begin; two cut rows are
     // noted before either is computed again)
     auto redo = [&](const Segment& s, uint32_t first_bit) {
         __syncthreads();
         if (const uint32_t odd = odd_rows >> first_bit & 0xffffu) {
-            if (s.r.n > 1)
 #pragma unroll 1
-                for (uint32_t row = warp; row < kDecRows; row += kDecWarps)
-                    if (odd >> row & 1u)
-                        attention_row<D, T>(a, s.b, s.r, (int32_t)((s.first + row) / a.group), s.kvh * a.group + (s.first + row) % a.group);
+            for (uint32_t row = warp; row < kDecRows; row += kDecWarps)
+                if (odd >> row & 1u)
+                    attention_row<D, T, false>(a, s.b, s.r, (int32_t)((s.first + row) / a.group),
+                                               s.kvh * a.group + (s.first + row) % a.group, s.sp.lo, s.r.kv - 1);
             __syncthreads();
             if (tid == 0)
                 odd_rows &= ~(0xffffu << first_bit);

@@ -742,16 +742,18 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
                 }
                 __syncwarp();
             }
-            odd = odd && my_row < rows;
+            odd = odd && my_row < rows && !isnan(l);  // a sum that is no number: the row sees such a score
             if (a.lse && my_row < rows)
                 a.lse[tok * a.lse_token + head] = l == 0.0f ? -INFINITY : __fmaf_rn(m, a.scale, ln_fast(l));
             // a row that came out infinite or NaN may owe it to a value that
-            // only later tokens see: again, key by key
+            // only other tokens see, or in BF16 to weights above one
             uint32_t again = __ballot_sync(0xffffffffu, odd);
+            __syncwarp();  // the results are read back
             while (again) {
                 const uint32_t i = (uint32_t)__ffs((int)again) - 1;
                 again &= again - 1;
-                attention_row<D, T>(a, b, r, (int32_t)((wrow + i) / a.group), kvh * a.group + (wrow + i) % a.group);
+                attention_row<D, T, !std::is_same<T, __half>::value>(a, b, r, (int32_t)((wrow + i) / a.group),
+                                                                     kvh * a.group + (wrow + i) % a.group, tiles.lo, tiles.last);
             }
         }
     }

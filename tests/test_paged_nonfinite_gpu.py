@@ -89,3 +89,30 @@ def test_values_inside_prompts(ops, name, bad, which):  # noqa: F811
     finite = torch.isfinite(want)
     within(got[finite], want[finite], tol[finite])
     assert not torch.isfinite(got[~finite]).any()
+
+
+@pytest.mark.parametrize("requests,dtype", [([(2048, 2048)], BF16), ([(2048, 2048)], F16), ([(2, 4096)] * 8, BF16), ([(40, 9000)], F16)])
+@pytest.mark.parametrize("which,share", [(2, 0.0), (1, 0.0), (1, 0.5)])
+def test_a_value_that_rows_see_costs_little(ops, requests, dtype, which, share):  # noqa: F811
+    """A NaN that makes most rows NaN, and rightly: they are not computed again key by key (160 to 800 times
+    the call's time). A check of the unseen values of each row is allowed: up to 64 keys' dependent loads a row of a
+    warp, 32 rows, at most 1 us a batch of eight: 0.3 ms for calls of 35 us and more, so 40 times bounds it."""
+    max_q = max(n for n, _ in requests)
+
+    def spent(made):
+        best = math.inf
+        for _ in range(4):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(4):
+                ops.attention(*made, max_q=max_q)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    made = make(requests, 16, 8, 128, 64, dtype)
+    plain = spent(made)
+    for b, (n, kv) in enumerate(requests):
+        poison(made, b, int(share * (kv - 1)), math.nan, which)
+    assert spent(made) < 40 * plain
