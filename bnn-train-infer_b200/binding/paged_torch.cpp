@@ -16,7 +16,6 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
-#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -309,18 +308,14 @@ PyObject* stream(PyObject*, PyObject* device) {
 // the last captured call's with its capture. Calls of unlike captures, and a
 // captured call and one outside, are ordered by whoever replays the graph.
 struct Order {
+    at::Tensor workspace;  // of `home`: what its allocator hands out again is ordered on that stream
+    c10::DeviceIndex device;
+    cudaStream_t home;
     cudaStream_t last;
     cudaStream_t captured;
     unsigned long long capture;  // 0: none yet
     cudaEvent_t event;
 };
-
-void drop_order(PyObject* capsule) {
-    if (Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, "bnn_b200.paged.order"))) {
-        cudaEventDestroy(u->event);
-        delete u;
-    }
-}
 
 void cuda_ok(cudaError_t e, const char* what) {
     if (e != cudaSuccess) {
@@ -345,33 +340,53 @@ void after(cudaStream_t now, cudaStream_t before, cudaEvent_t event) {
     cuda_ok(cudaStreamWaitEvent(now, event, 0), "workspace order");
 }
 
-// new_order(device) -> a workspace's order; its memory is of the current stream
-PyObject* new_order(PyObject*, PyObject* device) {
+// The workspace goes: its home stream first waits for the last call's. (A stream
+// that is gone by then has been drained by whoever destroyed it, or never was the
+// last; nothing may throw here.)
+void drop_order(PyObject* capsule) {
+    Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, "bnn_b200.paged.order"));
+    if (!u)
+        return;
+    int before = 0;
+    cudaGetDevice(&before);
+    cudaSetDevice(u->device);
+    if (u->last != u->home) {
+        if (capture_of(u->last) != 0 || capture_of(u->home) != 0)
+            new at::Tensor(u->workspace);  // no order to be had inside a capture: the memory stays taken
+        else if (cudaEventRecord(u->event, u->last) == cudaSuccess)
+            cudaStreamWaitEvent(u->home, u->event, 0);
+    }
+    cudaEventDestroy(u->event);
+    cudaSetDevice(before);
+    cudaGetLastError();
+    delete u;
+}
+
+// new_order(device, workspace) -> the order of a workspace just made on the current stream
+PyObject* new_order(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        const auto d = (c10::DeviceIndex)integer(device, "device");
+        if (n != 2)
+            refuse(BNN_EINVAL, "new_order: 2 arguments");
+        const auto d = (c10::DeviceIndex)integer(o[0], "device");
         const c10::cuda::CUDAGuard guard(d);
+        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
         cudaEvent_t event;
         cuda_ok(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "workspace order");
-        PyObject* capsule = PyCapsule_New(new Order{c10::cuda::getCurrentCUDAStream(d).stream(), nullptr, 0, event},
-                                          "bnn_b200.paged.order", drop_order);
-        return capsule;
+        return PyCapsule_New(new Order{tensor(o[1], "workspace"), d, now, now, nullptr, 0, event}, "bnn_b200.paged.order", drop_order);
     });
 }
 
-// order(order, device, workspace): the current stream's next work runs after the
-// work that used the workspace before; the memory, which belongs to the stream
-// it was allocated on, is not handed out again before this stream is done with it
+// order(order, device): the current stream's next work runs after the work that
+// used the workspace before
 PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 3)
-            refuse(BNN_EINVAL, "order: 3 arguments");
+        if (n != 2)
+            refuse(BNN_EINVAL, "order: 2 arguments");
         Order* u = static_cast<Order*>(PyCapsule_GetPointer(o[0], "bnn_b200.paged.order"));
         if (!u)
             return nullptr;
         const auto d = (c10::DeviceIndex)integer(o[1], "device");
-        const at::Tensor& workspace = tensor(o[2], "workspace");
-        const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(d);
-        const cudaStream_t now = current.stream();
+        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
         if (const unsigned long long capture = capture_of(now)) {
             // branches of one graph: an edge from the earlier to the later
             if (u->capture == capture && u->captured != now) {
@@ -386,7 +401,6 @@ PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
                 refuse(BNN_EBUSY, "the stream of the last call is being captured");
             const c10::cuda::CUDAGuard guard(d);
             after(now, u->last, u->event);
-            c10::cuda::CUDACachingAllocator::recordStream(workspace.storage().data_ptr(), current);
             u->last = now;
         }
         Py_RETURN_NONE;
@@ -410,7 +424,7 @@ PyMethodDef methods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"stream", stream, METH_O, nullptr},
-    {"new_order", new_order, METH_O, nullptr},
+    {"new_order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(new_order)), METH_FASTCALL, nullptr},
     {"order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(order)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -68,7 +68,7 @@ class Paged:
         if st != OK:
             raise BnnError(st, "bnn_b200_paged_workspace")
         self._workspace = torch.zeros(need.value, dtype=torch.uint8, device=f"cuda:{self._index}")
-        self._order = _paged_torch.new_order(self._index)
+        self._order = _paged_torch.new_order(self._index, self._workspace)
         self._turn = threading.Lock()
 
     def _check_open(self):
@@ -98,7 +98,7 @@ class Paged:
         if page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
         with self._turn:  # another thread's call comes before both or after both
-            _paged_torch.order(self._order, self._index, self._workspace)
+            _paged_torch.order(self._order, self._index)
             return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts,
                                           max_q, scale, window, sinks, out, f32, return_lse)
 

@@ -1,6 +1,9 @@
 """The workspace of the paged attention between streams and graph branches
 (marked gpu)."""
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 
@@ -129,7 +132,6 @@ def test_calls_on_many_streams(ops, rounds):  # noqa: F811
 
 def test_threads_share_a_workspace(ops):  # noqa: F811
     """Four threads, each on a stream of its own, call at once; every result is the lone call's."""
-    import sys
     import threading
     calls = some_calls()
     want = [ops.attention(*made, max_q=max_q) for made, max_q, _ in calls]
@@ -159,21 +161,54 @@ def test_threads_share_a_workspace(ops):  # noqa: F811
 
 
 def test_a_dropped_workspace_waits_for_other_streams(ops):  # noqa: F811
-    """An operators' object that goes while another stream works on its workspace: the memory is not handed out."""
+    """An operators' object that goes while another stream works on its workspace: what its own stream does
+    with the memory next comes after that."""
     from bnn_b200 import paged
     made, max_q, _ = some_calls()[0]
     want = ops.attention(*made, max_q=max_q)
     torch.cuda.synchronize()
     own = paged.Paged(ops.device)
-    size, at = own._workspace.numel(), own._workspace.data_ptr()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
         own.attention(*made, max_q=max_q)
         torch.cuda._sleep(200_000_000)  # a tenth of a second
         got = own.attention(*made, max_q=max_q)
+    assert torch.cuda.current_stream().query() and not side.query()
     del own
-    fresh = torch.empty(size, dtype=torch.uint8, device="cuda")
-    assert not side.query()
-    assert fresh.data_ptr() != at
+    assert not torch.cuda.current_stream().query() and not side.query()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_the_handles_stream_may_go_first():
+    """Calls on the device handle's own stream, the handle closed, then the operators' object dropped (in a
+    process of its own: an exception there would end it)."""
+    code = """if True:
+        import ctypes, gc, sys
+        sys.path[:0] = sys.argv[1:]
+        import torch
+        from bnn_b200 import accel, paged
+        from test_paged_gpu import BF16, make
+        for _ in range(2):
+            dev = accel.Device(0)
+            ops = paged.Paged(dev)
+            fn = dev.api.dll.bnn_b200_device_stream
+            fn.restype, fn.argtypes = ctypes.c_void_p, [ctypes.c_void_p]
+            made = make([(1, 900), (2, 50)], 4, 2, 128, 16, BF16)
+            want = ops.attention(*made, max_q=2)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(torch.cuda.ExternalStream(fn(dev.handle))):
+                got = ops.attention(*made, max_q=2)
+                ops.sync()
+            assert torch.equal(got, want)
+            dev.close()
+            del ops
+            gc.collect()
+            torch.zeros(1 << 25, device="cuda")
+            torch.cuda.synchronize()
+        print("through")
+    """
+    here = Path(__file__).resolve()
+    got = subprocess.run([sys.executable, "-c", code, str(here.parent), str(here.parents[1] / "bnn-train-infer_b200")], capture_output=True,
+                         text=True, timeout=300)
+    assert got.returncode == 0 and "through" in got.stdout, got.stderr[-2000:]
