@@ -163,8 +163,7 @@ BNN_Status BNN_DeviceOpen(uint32_t device_index, BNN_Device* out_device) {
     }
     d->last_status = d->d_status;
     d->single_jobs = 0;
-    d->inflight_count = 0;
-    d->inflight_overflow = false;
+    bnn::inflight_clear(d);
     *out_device = d;
     return BNN_OK;
 }
@@ -459,11 +458,6 @@ static void inflight_add(bnn_accel_device* d, uintptr_t begin, uintptr_t end) {
     d->inflight_count++;
 }
 
-static void inflight_clear(bnn_accel_device* d) {
-    d->inflight_count = 0;
-    d->inflight_overflow = false;
-}
-
 // Enqueues prep + contraction for a validated job on the device stream,
 // without synchronising. Rows are processed in chunks so the grid's y
 // dimension stays within limits; the prep pass over ALL rows runs before
@@ -663,7 +657,7 @@ BNN_Status bnn_b200_sync(BNN_Device device) {
         cudaGetLastError();
         return BNN_EIO;
     }
-    inflight_clear(device);
+    bnn::inflight_clear(device);
     const int st = *device->h_status;
     if (st & bnn::kStatusTimeout)
         return BNN_ETIMEOUT;
@@ -690,6 +684,8 @@ BNN_Status bnn_b200_test_wait_limit(BNN_Device device, uint64_t limit_ns, int st
     }
     return BNN_OK;
 }
+
+int bnn_b200_test_early_input(BNN_Device device) { return device && !device->inflight_overflow ? 1 : 0; }
 
 void* bnn_b200_device_stream(BNN_Device device) {
     return device ? static_cast<void*>(device->stream) : nullptr;

@@ -66,6 +66,12 @@ namespace bnn {
 constexpr int kPagedStatusWord = 3;  // index into bnn_accel_device::d_status
 constexpr int kStatusWords = 4;
 
+// The device's stream has been drained: no output is in flight.
+inline void inflight_clear(bnn_accel_device* d) {
+    d->inflight_count = 0;
+    d->inflight_overflow = false;
+}
+
 // Makes `ordinal` current for the lifetime of the guard, restoring the
 // caller's device afterwards.
 class DeviceGuard {

@@ -68,7 +68,7 @@ BNN_Status launch(void (*kernel)(Args), dim3 grid, uint32_t threads, size_t smem
 // The kernels here let their successor start early, and a one-row BNN job may
 // read its input before it waits for its predecessor (GemvArgs::early_input):
 // on the handle's own stream it must not while a paged call's outputs are in
-// flight.
+// flight, that is until bnn_b200_sync or bnn_b200_paged_sync has drained it.
 void outputs_in_flight(BNN_Device device, cudaStream_t stream) {
     if (stream == device->stream)
         device->inflight_overflow = true;
@@ -416,6 +416,8 @@ BNN_Status bnn_b200_paged_sync(BNN_Device device, void* stream) {
         cudaGetLastError();
         return BNN_EIO;
     }
+    if (s == device->stream)
+        bnn::inflight_clear(device);
     if (word & bnn::kStatusTimeout)
         return BNN_ETIMEOUT;
     return word ? BNN_ERANGE : BNN_OK;

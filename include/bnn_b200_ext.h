@@ -55,6 +55,11 @@ void* bnn_b200_buffer_device_ptr(BNN_Buffer buffer);
  * stream first. Call with (0, 0) to return to normal operation. */
 BNN_Status bnn_b200_test_wait_limit(BNN_Device device, uint64_t limit_ns, int starve_producer);
 
+/* Test hook: 1 if a one-row job enqueued now could read its input early (see
+ * bnn_b200_device_stream), 0 while kernels whose outputs are not listed one by
+ * one are in flight on the handle's stream. */
+int bnn_b200_test_early_input(BNN_Device device);
+
 /* GEMM_F32 that allocates nothing. No counterpart in the reference.
  *
  * For callers that cannot let a library allocate device memory while they
