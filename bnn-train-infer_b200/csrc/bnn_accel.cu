@@ -678,7 +678,7 @@ BNN_Status bnn_b200_test_wait_limit(BNN_Device device, uint64_t limit_ns, int st
         cudaMemcpyToSymbol(bnn::g_test_starve_producer, &starve, sizeof starve) != cudaSuccess ||
         bnn::set_test_hooks_engine(limit, starve) != cudaSuccess ||
         bnn::set_test_hooks_noalloc(limit, starve) != cudaSuccess ||
-        bnn::set_test_hooks_paged(limit, starve) != cudaSuccess) {
+        bnn::set_test_hooks_paged(limit, starve_producer) != cudaSuccess) {
         cudaGetLastError();
         return BNN_EIO;
     }

@@ -79,7 +79,8 @@ struct PrefillArgs {
     uint32_t every_request;  // 0: requests of few rows belong to the split kernel
 };
 
-// Test hook: a loader that issues nothing, so that every wait runs out.
+// Test hook: n > 0 is a loader that issues the copies of n - 1 tiles and no more,
+// so that the waits for the others run out.
 static __device__ int g_paged_starve = 0;
 
 // Instruction descriptor: D f32, A and B of one 16-bit type, M = 128; B K-major
@@ -319,7 +320,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
         const uint32_t per_tile = kPfKeys / page_rows;
         constexpr uint32_t kMostPages = kPfKeys / 16;
         uint32_t slot = 0, round = 0;
-        const bool starved = *reinterpret_cast<volatile int*>(&g_paged_starve) != 0;
+        const uint32_t fed = min(count, (uint32_t)*reinterpret_cast<volatile int*>(&g_paged_starve) - 1u);  // all of them where it is 0
         // this lane's page of tile t, or -1
         auto lookup = [&](uint32_t t) -> int32_t {
             const int32_t j = tiles.key(t) + (int32_t)(lane * page_rows);
@@ -328,7 +329,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
         };
         int32_t next = lookup(0);
 #pragma unroll 1
-        for (uint32_t t = 0; t < count; ++t) {
+        for (uint32_t t = 0; t < fed; ++t) {
             const int32_t page = next;
             next = lookup(t + 1);  // on its way while this tile's copies are issued
             const uint32_t parts = page_rows / 16;
@@ -345,8 +346,8 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
 #pragma unroll 1
             for (int which = 0; which < 2; ++which) {
                 if (round > 0)
-                    ok = wait(&empty[slot], (round - 1) & 1);
-                if (!ok || starved)
+                    ok = warp_wait(&empty[slot], (round - 1) & 1);
+                if (!ok)
                     break;
                 if (lane == 0) {
                     if (which == 0)
@@ -374,7 +375,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
                     ++round;
                 }
             }
-            if (!ok || starved) {
+            if (!ok) {
                 if (lane == 0)
                     atomicOr(a.status, kStatusTimeout);
                 break;
@@ -562,7 +563,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
 #pragma unroll 1
         for (uint32_t j = 0; j < steps; ++j) {
             const uint32_t t = kMode == kTurns ? 2 * j + stream : j;  // key tile
-            if (!(ok = wait(&s_ready[stream], j & 1)))
+            if (!(ok = warp_wait(&s_ready[stream], j & 1)))
                 break;
             tc_fence_after();
             uint32_t s[kPfKeys];
@@ -575,7 +576,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
                 // V rows that no row of this CTA sees become zeros before the first
                 // product with them (which waits for this stream's P)
                 const uint32_t slot = (2 * t + 1) % kStages;
-                if (!(ok = wait(&full[slot], ((2 * t + 1) / kStages) & 1)))
+                if (!(ok = warp_wait(&full[slot], ((2 * t + 1) / kStages) & 1)))
                     break;
                 unsigned char* v = ring + slot * kTileBytes;
 #pragma unroll 1
@@ -622,7 +623,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
             const bool grow = top > m && (top - m) * c > kSlack;  // also the first finite score
             if constexpr (kApart) {
                 // the last keys' product has read P and is in O
-                if (j > 0 && !(ok = wait(&o_ready[stream], (j - 1) & 1)))
+                if (j > 0 && !(ok = warp_wait(&o_ready[stream], (j - 1) & 1)))
                     break;
                 tc_fence_after();
             }
@@ -668,7 +669,7 @@ static __global__ void __launch_bounds__(PrefillShape<D, kMode>::kThreads, 1)
             l += (f2_lo(sum2[0]) + f2_hi(sum2[0])) + (f2_lo(sum2[1]) + f2_hi(sum2[1]));
         }
         // every product of stream s is in its O
-        auto finished = [&](uint32_t s, uint32_t n) { return n == 0 || (kApart ? wait(&o_ready[s], (n - 1) & 1) : wait(&s_ready[s], n & 1)); };
+        auto finished = [&](uint32_t s, uint32_t n) { return n == 0 || (kApart ? warp_wait(&o_ready[s], (n - 1) & 1) : warp_wait(&s_ready[s], n & 1)); };
         ok = ok && finished(stream, steps);
         float* joint = reinterpret_cast<float*>(ring);  // stream 1's O [column][row], then m and l
         if (kMode == kTurns) {

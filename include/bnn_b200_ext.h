@@ -51,8 +51,10 @@ void* bnn_b200_buffer_device_ptr(BNN_Buffer buffer);
  * one second) and, when starve_producer is non-zero, makes the contraction's
  * copy warps issue nothing, so the next GEMV/GEMV_F32/small-GEMM job's waits
  * for weight tiles run out and it returns BNN_ETIMEOUT without touching its
- * output. Affects every device in the process; waits for this handle's
- * stream first. Call with (0, 0) to return to normal operation. */
+ * output. The paged attention's tile kernel then issues the copies of
+ * starve_producer - 1 tiles of keys and no more. Affects every device in the
+ * process; waits for this handle's stream first. Call with (0, 0) to return to
+ * normal operation. */
 BNN_Status bnn_b200_test_wait_limit(BNN_Device device, uint64_t limit_ns, int starve_producer);
 
 /* Test hook: 1 if a one-row job enqueued now could read its input early (see
