@@ -284,7 +284,7 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
         return BNN_ENOTSUP;
     if (d.rotary_dim != 0 && (!d.cos || !d.sin || !aligned16(d.cos) || !aligned16(d.sin) || d.table_rows <= 0 || d.table_rows > kMaxCount))
         return BNN_EINVAL;
-    if (!(d.eps >= 0.0) || !std::isfinite(d.eps) || !aligned16(d.q_norm) || !aligned16(d.k_norm))
+    if (!(d.eps >= 0.0) || !std::isfinite((float)d.eps) || !aligned16(d.q_norm) || !aligned16(d.k_norm))
         return BNN_EINVAL;
     if (d.tokens == 0)
         return BNN_OK;
@@ -353,7 +353,8 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
         return BNN_EINVAL;
     if (d.heads / d.cache.kv_heads > BNN_PAGED_MAX_GROUP)
         return BNN_ENOTSUP;
-    if (d.window < 0 || d.sinks < 0 || !(d.scale > 0.0) || !std::isfinite((float)d.scale) || (float)d.scale == 0.0f)
+    const float scale_log2 = (float)(d.scale * 1.4426950408889634);
+    if (d.window < 0 || d.sinks < 0 || !(d.scale > 0.0) || !std::isfinite(scale_log2) || (float)d.scale == 0.0f)
         return BNN_EINVAL;
     if (d.table_width < 0 || d.table_width > kMaxCount || (d.batch > 1 && d.table_stride < d.table_width))
         return BNN_EINVAL;
@@ -385,7 +386,7 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
     a.sinks = (uint32_t)(d.sinks < kMaxCount ? d.sinks : kMaxCount);
     a.out_type = (uint32_t)d.out_type;
     a.scale = (float)d.scale;
-    a.scale_log2 = (float)(d.scale * 1.4426950408889634);
+    a.scale_log2 = scale_log2;
     a.partials = static_cast<float*>(d.workspace);
     a.group_counters = reinterpret_cast<int*>(static_cast<unsigned char*>(d.workspace) + partial_bytes(device));
     a.row_counters = a.group_counters + 2 * split_grid(device);

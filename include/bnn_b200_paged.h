@@ -124,7 +124,7 @@ typedef struct {
     int64_t table_stride, table_width;
     int64_t window, sinks;
     int64_t out_type; /* the cache's type or BNN_PAGED_F32 */
-    double scale;     /* finite and positive */
+    double scale;     /* positive; scale * log2(e) is a finite float */
 } BNN_PagedAttention;
 BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention* desc, void* stream);
 
