@@ -356,7 +356,7 @@ BNN_Status bnn_b200_paged_attention(BNN_Device device, const BNN_PagedAttention*
     const float scale_log2 = (float)(d.scale * 1.4426950408889634);
     if (d.window < 0 || d.sinks < 0 || !(d.scale > 0.0) || !std::isfinite(scale_log2) || (float)d.scale == 0.0f)
         return BNN_EINVAL;
-    if (d.table_width < 0 || d.table_width > kMaxCount || (d.batch > 1 && d.table_stride < d.table_width))
+    if (d.table_width < 0 || d.table_width > kMaxCount || (d.batch > 1 && d.table_stride < 0))
         return BNN_EINVAL;
     if (d.batch == 0 || d.tokens == 0 || d.max_q == 0)
         return BNN_OK;

@@ -114,7 +114,7 @@ typedef struct {
     const void* q;
     void* out;
     float* lse;
-    const int32_t* page_table; /* [batch][table_width], rows table_stride apart */
+    const int32_t* page_table; /* [batch][table_width], rows table_stride >= 0 apart (0: one row for all) */
     const int32_t* kv_lens;    /* [batch] */
     const int32_t* q_starts;   /* [batch + 1] */
     void* workspace;

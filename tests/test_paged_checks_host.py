@@ -61,3 +61,8 @@ def test_scale_is_checked_as_the_kernels_use_it(scale, want):
 @pytest.mark.parametrize("eps,want", [(0.0, accel.OK), (1e-60, accel.OK), (3e38, accel.OK), (1e39, accel.EINVAL), (-1e-9, accel.EINVAL)])
 def test_eps_is_checked_as_the_kernels_use_it(eps, want):
     assert append(eps=eps) == want
+
+
+@pytest.mark.parametrize("stride,want", [(3, accel.OK), (100, accel.OK), (2, accel.OK), (0, accel.OK), (-1, accel.EINVAL)])
+def test_requests_may_share_a_row_of_the_table(stride, want):
+    assert attention(batch=2, table_stride=stride) == want

@@ -78,3 +78,13 @@ def test_requests_without_tokens_may_hold_anything(ops):  # noqa: F811
     got = ops.attention(q, k, v, table, lens, starts, max_q=1)
     ops.sync()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_one_table_row_for_all_requests(ops, n):  # noqa: F811
+    """Requests that continue one prompt: the same pages for each, an expanded row."""
+    q, k, v, table, lens, starts = make([(n, 300)] * 4, 4, 2, 128, 16, BF16)
+    shared = table[1:2].expand(4, -1)
+    want = ops.attention(q, k, v, shared.contiguous(), lens, starts, max_q=n)
+    got, _ = check(ops, (q, k, v, shared, lens, starts))
+    assert torch.equal(got, want)
