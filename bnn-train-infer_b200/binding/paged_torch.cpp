@@ -123,8 +123,9 @@ void rows(const at::Tensor& x, const char* name, int64_t tokens, int64_t heads, 
     on_device(x, device, name);
     if (x.stride(2) != 1)
         refuse(BNN_EINVAL, "%s: the last dimension has to be adjacent", name);
-    *token_stride = x.stride(0);
-    *head_stride = x.stride(1);
+    // as in the cache, the stride of a dimension of one is free
+    *head_stride = heads > 1 ? x.stride(1) : dim;
+    *token_stride = tokens > 1 ? x.stride(0) : heads * dim;
 }
 
 // A call has been launched that writes x: what autograd saved of it is stale
