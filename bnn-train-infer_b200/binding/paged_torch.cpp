@@ -128,6 +128,16 @@ void rows(const at::Tensor& x, const char* name, int64_t tokens, int64_t heads, 
     *token_stride = tokens > 1 ? x.stride(0) : heads * dim;
 }
 
+// A result of the caller's: every value has a place of its own.
+const at::Tensor& given_out(PyObject* o) {
+    const at::Tensor& x = tensor(o, "out");
+    no_gradient(x, "out");
+    for (int64_t i = 0; i < x.dim(); ++i)
+        if (x.size(i) > 1 && x.stride(i) == 0)
+            refuse(BNN_EINVAL, "out: expanded, its rows share memory");
+    return x;
+}
+
 // A call has been launched that writes x: what autograd saved of it is stale
 // (inference tensors keep no count).
 void written(const at::Tensor& x) {
@@ -212,10 +222,9 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (o[15] == Py_None) {
             out = empty({d.tokens, d.heads, dim}, k_pages.scalar_type(), device);
         } else {
-            out = tensor(o[15], "out");
+            out = given_out(o[15]);
             if (out.scalar_type() != k_pages.scalar_type())
                 refuse(BNN_EINVAL, "out: the cache's type");
-            no_gradient(out, "out");
         }
         rows(out, "out", d.tokens, d.heads, dim, device, &d.out_token_stride, &d.out_head_stride);
         d.q_out = out.data_ptr();
@@ -268,8 +277,7 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         if (o[13] == Py_None) {
             out = empty({d.tokens, d.heads, dim}, PyObject_IsTrue(o[14]) == 1 ? at::kFloat : q.scalar_type(), device);
         } else {
-            out = tensor(o[13], "out");
-            no_gradient(out, "out");
+            out = given_out(o[13]);
         }
         rows(out, "out", d.tokens, d.heads, dim, device, &d.out_token_stride, &d.out_head_stride);
         d.out = out.data_ptr();

@@ -19,3 +19,18 @@ def test_a_dimension_of_one_may_have_any_stride(ops, tokens, heads, strides):  #
     odd = buffer.as_strided((tokens, heads, 128), strides, 1000)
     odd.copy_(made[0])
     check(ops, (odd, *made[1:]))
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 128), (3, 1, 128)])
+def test_an_expanded_result_is_refused(ops, shape):  # noqa: F811
+    """Its rows share memory: whichever is written last would stay."""
+    from bnn_b200 import accel
+    out = torch.empty(shape, dtype=BF16, device="cuda").expand(3, 4, 128)
+    made = make([(1, 40)] * 3, 4, 2, 128, 16, BF16)
+    at = torch.arange(3, dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.attention(*made, max_q=1, out=out),
+                 lambda: ops.append(*rows(3, 4, 2, 128, F32), None, None, at, at, *pool(2, 2, 16, 128, BF16), out=out)):
+        with pytest.raises(accel.BnnError) as e:
+            call()
+        assert e.value.status == accel.EINVAL
+    ops.sync()
