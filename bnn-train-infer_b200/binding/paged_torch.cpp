@@ -70,6 +70,15 @@ double number(PyObject* o, const char* name) {
     return v;
 }
 
+bool truth(PyObject* o, const char* name) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse(BNN_EINVAL, "%s: true or false is wanted", name);
+    }
+    return v == 1;
+}
+
 int64_t type_of(at::ScalarType t) {
     return t == at::kFloat ? BNN_PAGED_F32 : t == at::kBFloat16 ? BNN_PAGED_BF16 : t == at::kHalf ? BNN_PAGED_F16 : 0;
 }
@@ -217,7 +226,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
         d.q_norm = o[11] == Py_None ? nullptr : vector<float>(o[11], "q_norm", at::kFloat, dim, device);
         d.k_norm = o[12] == Py_None ? nullptr : vector<float>(o[12], "k_norm", at::kFloat, dim, device);
         d.eps = number(o[13], "eps");
-        d.interleaved = PyObject_IsTrue(o[14]) == 1;
+        d.interleaved = truth(o[14], "interleaved");
         at::Tensor out;
         if (o[15] == Py_None) {
             out = empty({d.tokens, d.heads, dim}, k_pages.scalar_type(), device);
@@ -275,14 +284,14 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         d.sinks = integer(o[12], "sinks");
         at::Tensor out, lse;
         if (o[13] == Py_None) {
-            out = empty({d.tokens, d.heads, dim}, PyObject_IsTrue(o[14]) == 1 ? at::kFloat : q.scalar_type(), device);
+            out = empty({d.tokens, d.heads, dim}, truth(o[14], "out_is_f32") ? at::kFloat : q.scalar_type(), device);
         } else {
             out = given_out(o[13]);
         }
         rows(out, "out", d.tokens, d.heads, dim, device, &d.out_token_stride, &d.out_head_stride);
         d.out = out.data_ptr();
         d.out_type = type_of(out.scalar_type());
-        const bool want_lse = PyObject_IsTrue(o[15]) == 1;
+        const bool want_lse = truth(o[15], "return_lse");
         if (want_lse) {
             lse = empty({d.tokens, d.heads}, at::kFloat, device);
             d.lse = static_cast<float*>(lse.data_ptr());

@@ -93,9 +93,9 @@ class Paged:
         f32 = False
         if out_dtype is not None:
             f32 = out_dtype == torch.float32
-            if not f32 and out_dtype != q.dtype or out is not None and out.dtype != out_dtype:
+            if not f32 and out_dtype != getattr(q, "dtype", None) or out is not None and getattr(out, "dtype", None) != out_dtype:
                 raise BnnError(EINVAL, "out_dtype: q's type or float32, and out's")
-        if page_table.shape[0] > self._max_batch:
+        if getattr(page_table, "ndim", 0) and page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
         with self._turn:  # another thread's call comes before both or after both
             _paged_torch.order(self._order, self._index)

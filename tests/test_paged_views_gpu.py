@@ -34,3 +34,24 @@ def test_an_expanded_result_is_refused(ops, shape):  # noqa: F811
             call()
         assert e.value.status == accel.EINVAL
     ops.sync()
+
+
+def test_arguments_of_another_kind_are_refused(ops):  # noqa: F811
+    """With the wrappers' error, and nothing launched: the result given stays as it is."""
+    from bnn_b200 import accel
+    q, k, v, table, lens, starts = made = make([(1, 40)], 4, 2, 128, 16, BF16)
+    at = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((1, 4, 128), 9.0, dtype=BF16, device="cuda")
+    many = torch.ones(2)  # no truth value
+    new = (*rows(1, 4, 2, 128, F32), None, None, at, at, *pool(2, 2, 16, 128, BF16))
+    for call in (lambda: ops.append(*new, out=out, interleaved=many), lambda: ops.attention(*made, max_q=1, out=out, return_lse=many),
+                 lambda: ops.attention(q, k, v, None, lens, starts, max_q=1, out=out),
+                 lambda: ops.attention(q, k, v, 3, lens, starts, max_q=1, out=out),
+                 lambda: ops.attention(None, k, v, table, lens, starts, max_q=1, out_dtype=BF16),
+                 lambda: ops.attention(*made, max_q=1, out=7, out_dtype=F32), lambda: ops.attention(*made, max_q=1.5, out=out),
+                 lambda: ops.attention(*made, max_q=1, out=out, scale="half"), lambda: ops.append(*new, out=out, eps=None)):
+        with pytest.raises(accel.BnnError) as e:
+            call()
+        assert e.value.status == accel.EINVAL
+    ops.sync()
+    assert (out == 9).all()
