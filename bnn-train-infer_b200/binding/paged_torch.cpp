@@ -11,6 +11,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <vector>
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -322,13 +323,14 @@ PyObject* stream(PyObject*, PyObject* device) {
     });
 }
 
+const cudaStream_t kNoStream = reinterpret_cast<cudaStream_t>(~(uintptr_t)0);  // compares unlike any
+
 // Who used a workspace last: the stream of the last call outside captures, and
 // the last captured call's with its capture. Calls of unlike captures, and a
 // captured call and one outside, are ordered by whoever replays the graph.
 struct Order {
-    at::Tensor workspace;  // of `home`: what its allocator hands out again is ordered on that stream
-    c10::DeviceIndex device;
-    cudaStream_t home;
+    at::Tensor workspace;
+    cudaStream_t home;  // where the allocator orders what it hands the memory out for next
     cudaStream_t last;
     cudaStream_t captured;
     unsigned long long capture;  // 0: none yet
@@ -358,39 +360,65 @@ void after(cudaStream_t now, cudaStream_t before, cudaEvent_t event) {
     cuda_ok(cudaStreamWaitEvent(now, event, 0), "workspace order");
 }
 
-// The workspace goes: its home stream first waits for the last call's. (A stream
-// that is gone by then has been drained by whoever destroyed it, or never was the
-// last; nothing may throw here.)
+// Workspaces whose object went while their last call, on another stream than
+// their own, may have been in flight. That stream may be gone as well, so it is
+// not asked (asking one that is gone ended the process): the memory stays here
+// until the next object on the device takes it over. Never destroyed, as CUDA
+// may be gone before this library.
+std::vector<at::Tensor>& left_behind() {
+    static auto* all = new std::vector<at::Tensor>;
+    return *all;
+}
+
 void drop_order(PyObject* capsule) {
     Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, "bnn_b200.paged.order"));
     if (!u)
         return;
-    int before = 0;
-    cudaGetDevice(&before);
-    cudaSetDevice(u->device);
-    if (u->last != u->home) {
-        if (capture_of(u->last) != 0 || capture_of(u->home) != 0)
-            new at::Tensor(u->workspace);  // no order to be had inside a capture: the memory stays taken
-        else if (cudaEventRecord(u->event, u->last) == cudaSuccess)
-            cudaStreamWaitEvent(u->home, u->event, 0);
-    }
+    if (u->last != u->home)
+        left_behind().push_back(u->workspace);
     cudaEventDestroy(u->event);
-    cudaSetDevice(before);
-    cudaGetLastError();
     delete u;
 }
 
-// new_order(device, workspace) -> the order of a workspace just made on the current stream
+// A left workspace of this size, all work on the device done.
+at::Tensor left_workspace(c10::DeviceIndex device, int64_t bytes, cudaStream_t now) {
+    auto& all = left_behind();
+    for (size_t i = 0; i < all.size(); ++i)
+        if (all[i].get_device() == device && all[i].numel() == bytes && capture_of(now) == 0) {
+            cuda_ok(cudaDeviceSynchronize(), "workspace");
+            at::Tensor x = all[i];
+            all.erase(all.begin() + (ptrdiff_t)i);
+            return x;
+        }
+    return at::Tensor();
+}
+
+// new_order(device, bytes) -> (a zeroed workspace, its order), of the current stream
 PyObject* new_order(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         if (n != 2)
             refuse(BNN_EINVAL, "new_order: 2 arguments");
         const auto d = (c10::DeviceIndex)integer(o[0], "device");
+        const int64_t bytes = integer(o[1], "bytes");
         const c10::cuda::CUDAGuard guard(d);
         const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
+        at::Tensor workspace = left_workspace(d, bytes, now);
+        const bool taken_over = workspace.defined();
+        if (!taken_over)
+            workspace = empty({bytes}, at::kByte, d);
+        cuda_ok(cudaMemsetAsync(workspace.data_ptr(), 0, (size_t)bytes, now), "workspace");
         cudaEvent_t event;
         cuda_ok(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "workspace order");
-        return PyCapsule_New(new Order{tensor(o[1], "workspace"), d, now, now, nullptr, 0, event}, "bnn_b200.paged.order", drop_order);
+        // one taken over belongs to a stream that is not known here: it is left behind again
+        Order* u = new Order{workspace, taken_over ? kNoStream : now, now, nullptr, 0, event};
+        PyObject* capsule = PyCapsule_New(u, "bnn_b200.paged.order", drop_order);
+        if (!capsule)
+            return nullptr;
+        PyObject* x = THPVariable_Wrap(workspace);
+        PyObject* both = x ? PyTuple_Pack(2, x, capsule) : nullptr;
+        Py_XDECREF(x);
+        Py_DECREF(capsule);
+        return both;
     });
 }
 

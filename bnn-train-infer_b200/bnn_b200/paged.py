@@ -67,8 +67,7 @@ class Paged:
         st = self._dll.bnn_b200_paged_workspace(device.handle, ctypes.byref(need))
         if st != OK:
             raise BnnError(st, "bnn_b200_paged_workspace")
-        self._workspace = torch.zeros(need.value, dtype=torch.uint8, device=f"cuda:{self._index}")
-        self._order = _paged_torch.new_order(self._index, self._workspace)
+        self._workspace, self._order = _paged_torch.new_order(self._index, need.value)
         self._turn = threading.Lock()
 
     def _check_open(self):

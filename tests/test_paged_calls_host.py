@@ -36,10 +36,9 @@ def recorded(monkeypatch):
     recorder = Recorder()
     real = paged._paged_torch
     monkeypatch.setattr(paged, "_paged_torch", types.SimpleNamespace(
-        bind=real.bind, stream=lambda d: 0, new_order=lambda d, w: None, order=recorder.order, attention=recorder.attention, append=recorder.append))
+        bind=real.bind, stream=lambda d: 0, new_order=lambda d, n: (None, None), order=recorder.order, attention=recorder.attention, append=recorder.append))
     dll = types.SimpleNamespace(bnn_b200_device_ordinal=lambda h: 0, bnn_b200_paged_workspace=lambda h, n: 0)
     monkeypatch.setattr(paged, "_bind", lambda: dll)
-    monkeypatch.setattr(paged.torch, "zeros", lambda *a, **k: None)
     device = types.SimpleNamespace(handle=types.SimpleNamespace(value=1))
     return paged.Paged(device), recorder
 

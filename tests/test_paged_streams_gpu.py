@@ -160,24 +160,42 @@ def test_threads_share_a_workspace(ops):  # noqa: F811
     ops.sync()
 
 
-def test_a_dropped_workspace_waits_for_other_streams(ops):  # noqa: F811
-    """An operators' object that goes while another stream works on its workspace: what its own stream does
-    with the memory next comes after that."""
+def test_a_dropped_workspace_is_not_handed_out(ops):  # noqa: F811
+    """An operators' object that goes while another stream works on its workspace: only the next such object
+    gets the memory, and only when that work is done."""
     from bnn_b200 import paged
     made, max_q, _ = some_calls()[0]
     want = ops.attention(*made, max_q=max_q)
+    for _ in range(3):
+        torch.cuda.synchronize()
+        own = paged.Paged(ops.device)
+        size, at = own._workspace.numel(), own._workspace.data_ptr()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            own.attention(*made, max_q=max_q)
+            torch.cuda._sleep(200_000_000)  # a tenth of a second
+            got = own.attention(*made, max_q=max_q)
+        del own
+        fresh = torch.empty(size, dtype=torch.uint8, device="cuda")
+        assert fresh.data_ptr() != at and not side.query()
+        heir = paged.Paged(ops.device)
+        assert heir._workspace.data_ptr() == at and side.query()
+        assert torch.equal(heir.attention(*made, max_q=max_q), want) and torch.equal(got, want)
+        del heir
+        ops.sync()
+
+
+def test_a_workspace_of_one_stream_goes_back(ops):  # noqa: F811
+    from bnn_b200 import paged
+    made, max_q, _ = some_calls()[0]
     torch.cuda.synchronize()
+    waiting = [paged.Paged(ops.device) for _ in range(8)]  # those that other tests left
     own = paged.Paged(ops.device)
-    side = torch.cuda.Stream()
-    with torch.cuda.stream(side):
-        own.attention(*made, max_q=max_q)
-        torch.cuda._sleep(200_000_000)  # a tenth of a second
-        got = own.attention(*made, max_q=max_q)
-    assert torch.cuda.current_stream().query() and not side.query()
+    size, at = own._workspace.numel(), own._workspace.data_ptr()
+    own.attention(*made, max_q=max_q)
     del own
-    assert not torch.cuda.current_stream().query() and not side.query()
-    torch.cuda.synchronize()
-    assert torch.equal(got, want)
+    assert torch.empty(size, dtype=torch.uint8, device="cuda").data_ptr() == at
+    del waiting
 
 
 def test_the_handles_stream_may_go_first():
@@ -189,7 +207,7 @@ def test_the_handles_stream_may_go_first():
         import torch
         from bnn_b200 import accel, paged
         from test_paged_gpu import BF16, make
-        for _ in range(2):
+        for _ in range(5):
             dev = accel.Device(0)
             ops = paged.Paged(dev)
             fn = dev.api.dll.bnn_b200_device_stream
