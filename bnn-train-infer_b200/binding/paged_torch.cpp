@@ -92,6 +92,8 @@ void on_device(const at::Tensor& x, int device, const char* name) {
 // These operators have no derivative: a tensor that wants one, of either mode, is
 // refused wherever it would be dropped.
 void no_gradient(const at::Tensor& x, const char* name) {
+    if (!x.unsafeGetTensorImpl()->autograd_meta())
+        return;  // most tensors here: ten such questions a call
     if (x.requires_grad() && c10::GradMode::is_enabled())
         refuse(BNN_EINVAL, "%s requires a gradient, and the paged operators have no backward pass", name);
     if (x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
@@ -180,6 +182,130 @@ PyObject* guarded(F&& f) {
     END_HANDLE_TH_ERRORS
 }
 
+constexpr char kOrderName[] = "bnn_b200.paged.order";
+const cudaStream_t kNoStream = reinterpret_cast<cudaStream_t>(~(uintptr_t)0);  // compares unlike any
+
+// Who used a workspace last. Calls of unlike captures, and a captured call and
+// one outside, are ordered by whoever replays the graph.
+struct Order {
+    at::Tensor workspace;
+    cudaStream_t home;  // where the allocator orders what it hands the memory out for next
+    cudaStream_t recent;  // the last call's
+    cudaStream_t last;    // the last call's outside captures
+    cudaStream_t captured;  // the last noted call's inside one,
+    unsigned long long capture;  // and its capture (0: none yet)
+    cudaEvent_t event;
+};
+
+void cuda_ok(cudaError_t e, const char* what) {
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        refuse(BNN_EIO, "%s: %s", what, cudaGetErrorString(e));
+    }
+}
+
+// The capture that `stream` is part of, 0 where it is in none.
+unsigned long long capture_of(cudaStream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream beside somebody's capture
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+void after(cudaStream_t now, cudaStream_t before, cudaEvent_t event) {
+    cuda_ok(cudaEventRecord(event, before), "workspace order");
+    cuda_ok(cudaStreamWaitEvent(now, event, 0), "workspace order");
+}
+
+// Workspaces whose object went while their last call, on another stream than
+// their own, may have been in flight. That stream may be gone as well, so it is
+// not asked (asking one that is gone ended the process): the memory stays here
+// until the next object on the device takes it over. Never destroyed, as CUDA
+// may be gone before this library.
+std::vector<at::Tensor>& left_behind() {
+    static auto* all = new std::vector<at::Tensor>;
+    return *all;
+}
+
+void drop_order(PyObject* capsule) {
+    Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, kOrderName));
+    if (!u)
+        return;
+    if (u->last != u->home)
+        left_behind().push_back(u->workspace);
+    cudaEventDestroy(u->event);
+    delete u;
+}
+
+// A left workspace of this size, all work on the device done.
+at::Tensor left_workspace(c10::DeviceIndex device, int64_t bytes, cudaStream_t now) {
+    auto& all = left_behind();
+    for (size_t i = 0; i < all.size(); ++i)
+        if (all[i].get_device() == device && all[i].numel() == bytes && capture_of(now) == 0) {
+            cuda_ok(cudaDeviceSynchronize(), "workspace");
+            at::Tensor x = all[i];
+            all.erase(all.begin() + (ptrdiff_t)i);
+            return x;
+        }
+    return at::Tensor();
+}
+
+// new_order(device, bytes) -> (a zeroed workspace, its order), of the current stream
+PyObject* new_order(PyObject*, PyObject* const* o, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 2)
+            refuse(BNN_EINVAL, "new_order: 2 arguments");
+        const auto d = (c10::DeviceIndex)integer(o[0], "device");
+        const int64_t bytes = integer(o[1], "bytes");
+        const c10::cuda::CUDAGuard guard(d);
+        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
+        at::Tensor workspace = left_workspace(d, bytes, now);
+        const bool taken_over = workspace.defined();
+        if (!taken_over)
+            workspace = empty({bytes}, at::kByte, d);
+        cuda_ok(cudaMemsetAsync(workspace.data_ptr(), 0, (size_t)bytes, now), "workspace");
+        cudaEvent_t event;
+        cuda_ok(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "workspace order");
+        // one taken over belongs to a stream that is not known here: it is left behind again
+        Order* u = new Order{workspace, taken_over ? kNoStream : now, now, now, nullptr, 0, event};
+        PyObject* capsule = PyCapsule_New(u, kOrderName, drop_order);
+        if (!capsule)
+            return nullptr;
+        PyObject* x = THPVariable_Wrap(workspace);
+        PyObject* both = x ? PyTuple_Pack(2, x, capsule) : nullptr;
+        Py_XDECREF(x);
+        Py_DECREF(capsule);
+        return both;
+    });
+}
+
+// The stream's next work runs after the work that used the workspace before.
+void in_order(Order* u, cudaStream_t now, c10::DeviceIndex device) {
+    if (now == u->recent && now == u->last)
+        return;  // whether it is captured by now or not (a query costs more than all else here)
+    const c10::cuda::CUDAGuard guard(device);
+    if (const unsigned long long capture = capture_of(now)) {
+        // branches of one graph: an edge from the earlier to the later; `last` may have
+        // been drawn into the capture since
+        if (u->capture == capture && u->captured != now)
+            after(now, u->captured, u->event);
+        if (u->last != now && capture_of(u->last) == capture)
+            after(now, u->last, u->event);
+        u->capture = capture;
+        u->captured = now;
+    } else if (u->last != now) {
+        // waiting for a stream that is being captured would draw this one in
+        if (capture_of(u->last) != 0)
+            refuse(BNN_EBUSY, "the stream of the last call is being captured");
+        after(now, u->last, u->event);
+        u->last = now;
+    }
+    u->recent = now;
+}
+
 // append(handle, device, q, k, v, cos, sin, positions, slots, k_pages, v_pages,
 //        q_norm, k_norm, eps, interleaved, out) -> q
 PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
@@ -251,12 +377,13 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
 }
 
 // attention(handle, device, workspace, q, k_pages, v_pages, page_table, kv_lens,
-//           q_starts, max_q, scale, window, sinks, out, out_is_f32, return_lse)
-// -> out or (out, lse)
+//           q_starts, max_q, scale, window, sinks, out, out_is_f32, return_lse, order)
+// -> out or (out, lse). The interpreter's lock is held from the order to the
+// launch: another thread's call on this workspace comes before both or after both.
 PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 16)
-            refuse(BNN_EINVAL, "attention: 16 arguments");
+        if (n != 17)
+            refuse(BNN_EINVAL, "attention: 17 arguments");
         const int device = (int)integer(o[1], "device");
         BNN_PagedAttention d = {};
         const at::Tensor &workspace = tensor(o[2], "workspace"), &q = tensor(o[3], "q"), &k_pages = tensor(o[4], "k_pages");
@@ -300,8 +427,12 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
         }
         d.workspace = workspace.data_ptr();
         d.workspace_bytes = (int64_t)workspace.nbytes();
-        const BNN_Status st = g_attention(reinterpret_cast<BNN_Device>(PyLong_AsVoidPtr(o[0])), &d,
-                                          c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream());
+        Order* order = static_cast<Order*>(PyCapsule_GetPointer(o[16], kOrderName));
+        if (!order)
+            return nullptr;
+        const cudaStream_t now = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+        in_order(order, now, (c10::DeviceIndex)device);
+        const BNN_Status st = g_attention(reinterpret_cast<BNN_Device>(PyLong_AsVoidPtr(o[0])), &d, now);
         if (st != BNN_OK)
             refuse(st, "bnn_b200_paged_attention");
         if (o[13] != Py_None)
@@ -323,136 +454,6 @@ PyObject* stream(PyObject*, PyObject* device) {
     });
 }
 
-const cudaStream_t kNoStream = reinterpret_cast<cudaStream_t>(~(uintptr_t)0);  // compares unlike any
-
-// Who used a workspace last: the stream of the last call outside captures, and
-// the last captured call's with its capture. Calls of unlike captures, and a
-// captured call and one outside, are ordered by whoever replays the graph.
-struct Order {
-    at::Tensor workspace;
-    cudaStream_t home;  // where the allocator orders what it hands the memory out for next
-    cudaStream_t last;
-    cudaStream_t captured;
-    unsigned long long capture;  // 0: none yet
-    cudaEvent_t event;
-};
-
-void cuda_ok(cudaError_t e, const char* what) {
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        refuse(BNN_EIO, "%s: %s", what, cudaGetErrorString(e));
-    }
-}
-
-// The capture that `stream` is part of, 0 where it is in none.
-unsigned long long capture_of(cudaStream_t stream) {
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
-        cudaGetLastError();  // the legacy stream beside somebody's capture
-        return 0;
-    }
-    return status == cudaStreamCaptureStatusActive ? id : 0;
-}
-
-void after(cudaStream_t now, cudaStream_t before, cudaEvent_t event) {
-    cuda_ok(cudaEventRecord(event, before), "workspace order");
-    cuda_ok(cudaStreamWaitEvent(now, event, 0), "workspace order");
-}
-
-// Workspaces whose object went while their last call, on another stream than
-// their own, may have been in flight. That stream may be gone as well, so it is
-// not asked (asking one that is gone ended the process): the memory stays here
-// until the next object on the device takes it over. Never destroyed, as CUDA
-// may be gone before this library.
-std::vector<at::Tensor>& left_behind() {
-    static auto* all = new std::vector<at::Tensor>;
-    return *all;
-}
-
-void drop_order(PyObject* capsule) {
-    Order* u = static_cast<Order*>(PyCapsule_GetPointer(capsule, "bnn_b200.paged.order"));
-    if (!u)
-        return;
-    if (u->last != u->home)
-        left_behind().push_back(u->workspace);
-    cudaEventDestroy(u->event);
-    delete u;
-}
-
-// A left workspace of this size, all work on the device done.
-at::Tensor left_workspace(c10::DeviceIndex device, int64_t bytes, cudaStream_t now) {
-    auto& all = left_behind();
-    for (size_t i = 0; i < all.size(); ++i)
-        if (all[i].get_device() == device && all[i].numel() == bytes && capture_of(now) == 0) {
-            cuda_ok(cudaDeviceSynchronize(), "workspace");
-            at::Tensor x = all[i];
-            all.erase(all.begin() + (ptrdiff_t)i);
-            return x;
-        }
-    return at::Tensor();
-}
-
-// new_order(device, bytes) -> (a zeroed workspace, its order), of the current stream
-PyObject* new_order(PyObject*, PyObject* const* o, Py_ssize_t n) {
-    return guarded([&]() -> PyObject* {
-        if (n != 2)
-            refuse(BNN_EINVAL, "new_order: 2 arguments");
-        const auto d = (c10::DeviceIndex)integer(o[0], "device");
-        const int64_t bytes = integer(o[1], "bytes");
-        const c10::cuda::CUDAGuard guard(d);
-        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
-        at::Tensor workspace = left_workspace(d, bytes, now);
-        const bool taken_over = workspace.defined();
-        if (!taken_over)
-            workspace = empty({bytes}, at::kByte, d);
-        cuda_ok(cudaMemsetAsync(workspace.data_ptr(), 0, (size_t)bytes, now), "workspace");
-        cudaEvent_t event;
-        cuda_ok(cudaEventCreateWithFlags(&event, cudaEventDisableTiming), "workspace order");
-        // one taken over belongs to a stream that is not known here: it is left behind again
-        Order* u = new Order{workspace, taken_over ? kNoStream : now, now, nullptr, 0, event};
-        PyObject* capsule = PyCapsule_New(u, "bnn_b200.paged.order", drop_order);
-        if (!capsule)
-            return nullptr;
-        PyObject* x = THPVariable_Wrap(workspace);
-        PyObject* both = x ? PyTuple_Pack(2, x, capsule) : nullptr;
-        Py_XDECREF(x);
-        Py_DECREF(capsule);
-        return both;
-    });
-}
-
-// order(order, device): the current stream's next work runs after the work that
-// used the workspace before
-PyObject* order(PyObject*, PyObject* const* o, Py_ssize_t n) {
-    return guarded([&]() -> PyObject* {
-        if (n != 2)
-            refuse(BNN_EINVAL, "order: 2 arguments");
-        Order* u = static_cast<Order*>(PyCapsule_GetPointer(o[0], "bnn_b200.paged.order"));
-        if (!u)
-            return nullptr;
-        const auto d = (c10::DeviceIndex)integer(o[1], "device");
-        const cudaStream_t now = c10::cuda::getCurrentCUDAStream(d).stream();
-        if (const unsigned long long capture = capture_of(now)) {
-            // branches of one graph: an edge from the earlier to the later
-            if (u->capture == capture && u->captured != now) {
-                const c10::cuda::CUDAGuard guard(d);
-                after(now, u->captured, u->event);
-            }
-            u->capture = capture;
-            u->captured = now;
-        } else if (u->last != now) {
-            // waiting for a stream that is being captured would draw this one in
-            if (capture_of(u->last) != 0)
-                refuse(BNN_EBUSY, "the stream of the last call is being captured");
-            const c10::cuda::CUDAGuard guard(d);
-            after(now, u->last, u->event);
-            u->last = now;
-        }
-        Py_RETURN_NONE;
-    });
-}
-
 // bind(address of bnn_b200_paged_append, of bnn_b200_paged_attention, BnnError)
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *f, *g, *error;
@@ -471,7 +472,6 @@ PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"stream", stream, METH_O, nullptr},
     {"new_order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(new_order)), METH_FASTCALL, nullptr},
-    {"order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(order)), METH_FASTCALL, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

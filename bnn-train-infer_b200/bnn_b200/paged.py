@@ -18,7 +18,6 @@ torch.no_grad(). The tensors are read and checked in binding/paged_torch.cpp, bu
 file by the package Makefile; without it the import raises.
 """
 import ctypes
-import threading
 
 import torch
 
@@ -68,7 +67,6 @@ class Paged:
         if st != OK:
             raise BnnError(st, "bnn_b200_paged_workspace")
         self._workspace, self._order = _paged_torch.new_order(self._index, need.value)
-        self._turn = threading.Lock()
 
     def _check_open(self):
         if not self.device.handle:
@@ -96,10 +94,8 @@ class Paged:
                 raise BnnError(EINVAL, "out_dtype: q's type or float32, and out's")
         if getattr(page_table, "ndim", 0) and page_table.shape[0] > self._max_batch:
             raise BnnError(ENOTSUP, f"more than {self._max_batch} requests")
-        with self._turn:  # another thread's call comes before both or after both
-            _paged_torch.order(self._order, self._index)
-            return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts,
-                                          max_q, scale, window, sinks, out, f32, return_lse)
+        return _paged_torch.attention(self._handle, self._index, self._workspace, q, k_pages, v_pages, page_table, kv_lens, q_starts, max_q,
+                                      scale, window, sinks, out, f32, return_lse, self._order)
 
     def sync(self):
         """Waits for the current stream; raises what the calls since the last sync recorded

@@ -38,18 +38,21 @@ def captured_edges(graph):
     return kernels, set(zip(first, second))
 
 
-def fork(ops, calls):  # noqa: F811
-    """A graph with each call on a branch of its own."""
+def fork(ops, calls, stream=None, also_on_main=False):  # noqa: F811
+    """A graph with each call on a branch of its own (captured from `stream`; the first once more at the end)."""
     graph = torch.cuda.CUDAGraph(keep_graph=True)
     sides = [torch.cuda.Stream() for _ in calls[1:]]
     torch.cuda.synchronize()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(graph, stream=stream):
         main = torch.cuda.current_stream()
         for side in sides:
             side.wait_stream(main)
         for stream, (made, max_q, out) in zip([main] + sides, calls):
             with torch.cuda.stream(stream):
                 ops.attention(*made, max_q=max_q, out=out)
+        if also_on_main:
+            made, max_q, out = calls[0]
+            ops.attention(*made, max_q=max_q, out=out)
         for side in sides:
             main.wait_stream(side)
     return graph
@@ -63,15 +66,21 @@ def some_calls():
     return calls
 
 
-def test_branches_of_a_graph_are_ordered(ops):  # noqa: F811
+@pytest.mark.parametrize("used_before", [False, True])
+@pytest.mark.parametrize("also_on_main", [False, True])
+def test_branches_of_a_graph_are_ordered(ops, used_before, also_on_main):  # noqa: F811
     for _ in range(2):  # also in a second capture
-        graph = fork(ops, some_calls())
+        calls, stream = some_calls(), torch.cuda.Stream()
+        if used_before:  # the stream of the last call outside is the one that is captured then
+            with torch.cuda.stream(stream):
+                ops.attention(*calls[0][0], max_q=calls[0][1])
+        graph = fork(ops, calls, stream, also_on_main)
         kernels, edges = captured_edges(graph)
-        assert len(kernels) == 3
+        assert len(kernels) == 3 + also_on_main
         reach = {k: {b for a, b in edges if a == k} for k in kernels}
         for _ in kernels:
             reach = {k: r.union(*(reach[x] for x in r)) for k, r in reach.items()}
-        assert sorted(len(r) for r in reach.values()) == [0, 1, 2]
+        assert sorted(len(r) for r in reach.values()) == list(range(len(kernels)))
         del graph
 
 
@@ -101,11 +110,11 @@ def test_a_stream_under_capture_is_not_waited_for(ops):  # noqa: F811
     with torch.cuda.stream(side):
         want = ops.attention(*made, max_q=max_q)
     torch.cuda.synchronize()
-    other = torch.cuda.Stream()
+    other, another = torch.cuda.Stream(), torch.empty_like(out)
     with torch.cuda.graph(graph, stream=side):
         ops.attention(*made, max_q=max_q, out=out)
         with torch.cuda.stream(other), pytest.raises(accel.BnnError) as e:
-            ops.attention(*made, max_q=max_q, out=torch.empty(0))
+            ops.attention(*made, max_q=max_q, out=another)
         assert e.value.status == accel.EBUSY
     graph.replay()
     torch.cuda.synchronize()
