@@ -76,7 +76,11 @@ void outputs_in_flight(BNN_Device device, cudaStream_t stream) {
 
 // ---- append
 
-constexpr uint64_t kAppendWide = 148 * 64;  // (token, head) rows: more than the warps that fit the GPU at once
+// (token, head) rows: more than the warps that fit the GPU's 148 SMs at once. One
+// head a warp and four, 32 heads from FP32: 32 tokens 1.7 and 1.9 us, 64 2.0 and
+// 1.9, 256 (8192 rows) 3.3 and 2.9, 512 4.8 and 3.4, 8192 69 and 32 (in a graph):
+// the rule holds on to one head longer than it pays, by 0.5 us at most.
+constexpr uint64_t kAppendWide = 148 * 64;
 
 template <int D, typename S, typename T, int kHeads>
 BNN_Status launch_append(const AppendArgs& a, bool interleaved, cudaStream_t stream) {
@@ -91,8 +95,9 @@ BNN_Status launch_append(const AppendArgs& a, bool interleaved, cudaStream_t str
 template <int D, typename S, typename T>
 BNN_Status append_heads(const AppendArgs& a, bool interleaved, cudaStream_t stream) {
     // Four heads a warp where that still fills the GPU (their loads overlap and
-    // share the rotation's factors: 8192 tokens of 32 heads: 64 us with two, 54 with four, 55 with eight before the instructions were cut, 36 after), one
-    // where the call is short and more warps are the faster way through it.
+    // share the rotation's factors; two and eight were slower: 64 and 55 us against
+    // 54 for 8192 tokens of 32 heads at the time), one where the call is short and
+    // more warps are the faster way through it.
     const uint64_t rows = (uint64_t)a.tokens * (a.heads + 2 * a.c.kv_heads);
     return rows >= kAppendWide ? launch_append<D, S, T, 4>(a, interleaved, stream) : launch_append<D, S, T, 1>(a, interleaved, stream);
 }
@@ -212,13 +217,25 @@ BNN_Status launch_tiles(BNN_Device device, const AttnArgs& a, cudaStream_t strea
                   stream, args);
 }
 
-constexpr uint32_t kMixedCache = 1024;  // positions
+// Positions from which requests of few rows get the split kernel beside tiles for
+// the others. Tiles alone and both, in a graph: 60 single tokens behind 400 and a
+// prompt of 512 66 and 46 us, behind 1000 97 and 67, behind 4000 277 and 179; but
+// 8 single tokens and 100 tokens behind 400 12 and 25 us, behind 1000 19 and 31,
+// behind 4000 56 and 81, where one kernel waits for the other and neither fills
+// the GPU. How many requests there are of a kind only the device knows.
+constexpr uint32_t kMixedCache = 1024;
+// Positions up to which one stream works a tile of rows, in place of two in turn:
+// prompts of 256 9.1 and 10.6 us, 512 12.3 and 12.9, 640 13.8 both, 768 15.5 and
+// 15.0, 1024 18.6 and 17.1; 100 tokens behind 512 12.2 and 12.8, behind 768 15.3
+// and 14.6.
 constexpr uint32_t kTurnsCache = 512;
 
 template <int D, typename T>
 BNN_Status attention_typed(BNN_Device device, AttnArgs a, cudaStream_t stream) {
     // Requests of few rows go to the split kernel, the others to the tiles; each
-    // kernel finds its own. Where one of them can serve the whole call it goes
+    // kernel finds its own. The lengths are on the device: what a cache can be
+    // long is the page table's width here, so a table that is wider than its
+    // requests need can bring the other kernel, or both. Where one of them can serve the whole call it goes
     // alone (a launch that finds nothing to do costs 2 us): the split kernel if
     // no request has more than 16 rows, the tiles if every cache is short (eight
     // key tiles at most), either one for a single request.
@@ -236,9 +253,8 @@ BNN_Status attention_typed(BNN_Device device, AttnArgs a, cudaStream_t stream) {
     }
     const uint64_t pairs = (((uint64_t)a.tokens * a.group) / (2 * kPfRows) + a.batch) * a.c.kv_heads;
     // Two row tiles in a CTA while such pairs fill the GPU; else one, with two
-    // streams over its keys where there are enough of them (one stream and two:
-    // 256 tokens behind 8192 positions 118 and 93 us, 100 behind 1000 22 and 20 us,
-    // a 512-token prompt 12.7 and 13.2 us, eight of up to 64 tokens 8.0 and 9.2 us).
+    // streams over its keys where there are enough of them (kTurnsCache; 256 tokens
+    // behind 8192 positions 118 us with one stream and 93 with two).
     if (pairs >= (uint64_t)device->sm_count)
         return launch_tiles<D, T, kPair>(device, a, stream, !mixed);
     return ((uint64_t)a.table_width << a.c.page_shift) > kTurnsCache ? launch_tiles<D, T, kTurns>(device, a, stream, !mixed)

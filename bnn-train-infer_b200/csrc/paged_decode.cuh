@@ -35,8 +35,15 @@ constexpr uint32_t kDecThreads = kDecWarps * 32;
 constexpr uint32_t kDecTile = 16;                     // keys of a warp's step
 constexpr uint32_t kDecBlock = kDecTile * kDecWarps;  // keys of a CTA's step
 constexpr uint32_t kDecPerSm = 2;                     // CTAs an SM holds: 192 KB of ring
-constexpr uint32_t kWholeBlocks = 8;                  // a join costs as much as these blocks
-constexpr uint32_t kMinShare = 4;                     // units (below)
+// Rows of this many blocks are not cut: a join costs about as much as they do. With
+// 4, 8 and 16: one request of 600 positions (8 KV heads) 10.3, 10.3 and 14.7 us,
+// 32 of 300 13.4, 10.8 and 10.8, 32 of 600 18.7, 18.8 and 16.1, 61 ragged ones of
+// up to 3000 57.6, 58.4 and 64.5.
+constexpr uint32_t kWholeBlocks = 8;
+// Units (below) of a share at least. With 2, 4 and 8: one request of 600 positions
+// 8.8, 10.2 and 13.4 us, of 4000 11.6, 13.3 and 15.5, 8 of 600 10.3, 11.4 and
+// 14.8, 8 of 1000 12.1, 12.1 and 15.5; longer calls are alike.
+constexpr uint32_t kMinShare = 4;
 // A row's fixed work (its queries, the pipeline's start, the joint sum) in
 // units of the time a block takes: shares are equal in blocks plus rows (61
 // ragged requests: 132 us with 0, 78 with 2, 73 with 3 on the same code).
@@ -56,6 +63,8 @@ struct DecodeShape {
     static_assert(kDecRows * D * 4 <= kStageBytes, "a warp's O fits a stage");
 };
 
+// The ring, then the requests. From some 1000 requests on (16 bytes each) only one
+// CTA fits an SM: 1000 requests of 500 positions run at 4.3 TB/s, 1100 at 3.1.
 inline size_t decode_smem(uint32_t ring, uint32_t batch) { return ring + ((size_t)batch + 1) * (4 + sizeof(Request)); }
 
 // The 64-key blocks of a request that some of its new tokens see: the sinks'
@@ -509,6 +518,10 @@ static __global__ void __launch_bounds__(kDecThreads, kDecPerSm) attention_split
                     }
                 }
             }
+            // The weights are rounded to the cache's type: both operands of a product have
+            // one. The sum keeps them unrounded, so that it brings no rounding of its own
+            // into the result and lse. An F16 weight below 2^-25 of the row's largest so
+            // far is lost to the product.
             uint32_t pf[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {

@@ -66,7 +66,7 @@ typedef struct {
  * up to head_dim. A position outside the table leaves the token's q_out rows
  * zero and stores nothing, a slot outside the cache stores nothing; both make
  * the next bnn_b200_paged_sync return BNN_ERANGE. Two tokens of one call
- * must not share a slot. q_out's rows lie on 8-byte boundaries; q, k and v may
+ * must not share a slot. Outputs overlap no input. q_out's rows lie on 8-byte boundaries; q, k and v may
  * lie anywhere (16-byte rows load faster). */
 typedef struct {
     BNN_PagedCache cache;
@@ -107,8 +107,10 @@ BNN_Status bnn_b200_paged_append(BNN_Device device, const BNN_PagedAppend* desc,
  * kv_len below zero or above table_width * page_size, stay unwritten and the
  * next bnn_b200_paged_sync returns BNN_ERANGE. workspace: bnn_b200_paged_workspace
  * bytes, zeroed once before its first use and used by one call at a time
- * (calls on one stream may share it). Results do not depend on what else is
- * in flight: sums are joined in a fixed order. */
+ * (calls on one stream may share it). Outputs overlap no input. Results do not
+ * depend on what else is in flight: sums are joined in a fixed order. Which
+ * kernels serve a call goes by the sizes given here, the longest cache by
+ * table_width: a table no wider than its requests need is the faster one. */
 typedef struct {
     BNN_PagedCache cache;
     const void* q;
