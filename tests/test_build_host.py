@@ -53,3 +53,16 @@ def test_binding_follows_torch(tmp_path):
     stamp.write_text("another torch\n")
     os.utime(made, (stamp.stat().st_mtime - 10,) * 2)
     assert builds() == 2
+
+
+@pytest.mark.parametrize("checkout", [False, True])
+def test_checkers_are_built_where_the_reference_is(tmp_path, monkeypatch, checkout):
+    """An empty folder in its place is no reason to fail."""
+    import __graft_entry__ as entry
+    if checkout:
+        (tmp_path / "bnn-accelerator").mkdir()
+    ran = []
+    monkeypatch.setattr(entry, "REFERENCE", tmp_path)
+    monkeypatch.setattr(entry.subprocess, "run", lambda command, **kw: ran.append(command))
+    entry.build()
+    assert any("ref" in command for command in ran) == checkout
